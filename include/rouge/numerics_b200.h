@@ -430,6 +430,41 @@ int rouge_b200_gemm_f16(int M, int N, int K, const uint16_t *A, const uint16_t *
                         int b_layout, int is_bf16, void *C, int ldc, int out_type,
                         void *stream);
 
+/* GEMMs with bias, activation and residual in the epilogue (no reference
+ * counterpart: its callers make separate passes over C). With v the value
+ * rouge_b200_gemm_i8 / _e4m3 / _f16 would give in f32:
+ *   C[m][n] = round(act(v + bias[n]) + residual[m][n])
+ * all in f32 and rounded once to the output type. bias (f32 [N]) and
+ * residual (rows of ldr >= N elements of residual_type) may each be NULL.
+ * residual may be C itself (same address, pitch and element type); any
+ * other overlap with C is not allowed. act: gelu is v/2 (1 + erf(v/sqrt 2)),
+ * silu v / (1 + e^-v). Layouts, alignment and scales as in the plain
+ * entries; residual and bias need only their elements' alignment (16 bytes
+ * is faster). out_type F32 or BF16 (I32: EINVAL). The struct is read before
+ * the call returns. */
+#define ROUGE_B200_ACT_NONE 0
+#define ROUGE_B200_ACT_RELU 1
+#define ROUGE_B200_ACT_GELU 2
+#define ROUGE_B200_ACT_SILU 3
+typedef struct RougeB200Epilogue {
+  const float *bias;    /* [N] or NULL */
+  const void *residual; /* [M][ldr] or NULL */
+  long long ldr;
+  int residual_type;    /* ROUGE_B200_T_F32, _F16 or _BF16 */
+  int act;              /* ROUGE_B200_ACT_* */
+} RougeB200Epilogue;
+int rouge_b200_gemm_i8_fused(int M, int N, int K, const int8_t *A, const int8_t *B, int b_layout,
+                             const float *scales_a, int a_rows, const float *scales_b, int b_cols,
+                             const RougeB200Epilogue *epilogue, void *C, int ldc, int out_type,
+                             void *stream);
+int rouge_b200_gemm_e4m3_fused(int M, int N, int K, const uint8_t *A, const uint8_t *B,
+                               int b_layout, const float *scale_a, const float *scale_b,
+                               const RougeB200Epilogue *epilogue, void *C, int ldc, int out_type,
+                               void *stream);
+int rouge_b200_gemm_f16_fused(int M, int N, int K, const uint16_t *A, const uint16_t *B,
+                              int b_layout, int is_bf16, const RougeB200Epilogue *epilogue,
+                              void *C, int ldc, int out_type, void *stream);
+
 /* Implicit-GEMM 2-D convolution on tcgen05 (kind::f16), the B200 form of
  * rouge_conv2d_f32 / rouge_conv_implicit_f32 (numerics.h:76-79,106-109;
  * conv.cpp:26-66): cross-correlation with symmetric stride and zero
@@ -575,6 +610,86 @@ int rouge_b200_transformer_block(int S, int D, int Hq, int Hkv, int Dq, int Dk, 
                                  const float *wgate, const float *wup, const float *wdown, int Dff,
                                  float rope_theta, float rms_eps, float *out, void *workspace,
                                  size_t workspace_bytes, void *stream);
+
+/* Residual addition, RMS norm and 8-bit output in one launch (no reference
+ * counterpart as one call; the steps are transformer.cpp:33-40 and the
+ * quantizers). For each row of x[rows][cols] (row pitch ldx elements):
+ *   h = x + residual, rounded to `type` and written to h_out
+ *       (residual and h_out both NULL: h = x)
+ *   y = (float)(h / sqrt(mean(h^2) + eps)) * w[cols]     as rouge_rmsnorm
+ *   codes[rows][cols], scales:
+ *     ROUGE_B200_Q_I8_ROWS  rouge_b200_quantize_i8_rows of y: scales f32
+ *                           [rows] (cols % 4 == 0)
+ *     ROUGE_B200_Q_MX_E4M3  rouge_b200_mx_quantize(E4M3) of y: scales
+ *                           uint8 [rows][cols / 32] (cols % 32 == 0)
+ * type: ROUGE_B200_T_F32, _F16 or _BF16, of x, residual and h_out, whose
+ * rows need 16-byte alignment (8 bytes for the 16-bit types; 16 is faster);
+ * w f32 [cols], 16-byte aligned. h_out may be x or residual itself, with
+ * that array's pitch. rows == 0 does nothing. */
+#define ROUGE_B200_Q_I8_ROWS 0
+#define ROUGE_B200_Q_MX_E4M3 1
+int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const void *residual,
+                                 long long ldr, const float *w, float eps, int rows, int cols,
+                                 int type, void *h_out, long long ldh, int out_fmt, void *codes,
+                                 void *scales, void *stream);
+
+/* A paged cache of keys and values held in 4 bits (no reference
+ * counterpart; its caches are f32 or e4m3). Token slot p * page + i is
+ * position i of page p. Per slot and K/V head, Dh values in blocks of 16:
+ * packed e2m1 codes (lower index in the low nibble) and one UE4M3 scale per
+ * block, 4.5 bits per value; value = code * scale * gs[head].
+ *   k_codes, v_codes    [pages][Hkv][page][Dh / 2]   bytes
+ *   k_scales, v_scales  [pages][Hkv][page][Dh / 16]  bytes
+ *   gs_k, gs_v          [Hkv] f32 > 0, or NULL for 1
+ * page a multiple of 16, Dh a multiple of 16 up to 256, arrays 16-byte
+ * aligned, pages * page below 2^31; otherwise ROUGE_B200_EUNSUPPORTED. All
+ * pointers are device pointers; the struct itself is read before a call
+ * returns. */
+typedef struct RougeB200KV4 {
+  uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const float *gs_k, *gs_v;
+  int pages, page, Hkv, Dh;
+} RougeB200KV4;
+
+/* Writes tokens: K, V [T][Hkv][Dh] of `type` (F32, F16 or BF16; token
+ * pitches ldk, ldv >= Hkv * Dh elements; 16-byte aligned rows) into slots[T]
+ * (device int32). Per block: scale = e4m3(amax / (6 gs)), code =
+ * e2m1(x / (scale gs)), both to nearest even and saturating; a zero scale
+ * gives zero codes, a NaN is left out of amax and coded +6. A negative slot
+ * skips its token. Slots of one call must differ: the content of a slot
+ * given twice is undefined. A slot >= pages * page is skipped and makes the
+ * next rouge_b200_sync_status return ROUGE_B200_EINVAL. */
+int rouge_b200_kv4_write(const RougeB200KV4 *cache, const void *K, long long ldk, const void *V,
+                         long long ldv, int type, int T, const int *slots, void *stream);
+/* Reads tokens back: the values of slots[T], rounded once to `type`, into
+ * K, V (as above). Rows of negative or too large slots are left as they
+ * were (the latter reported as in rouge_b200_kv4_write). */
+int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void *V, long long ldv,
+                        int type, int T, const int *slots, void *stream);
+
+/* Attention of new tokens over the cache. B sequences; sequence b has
+ * kv_len[b] keys (device int32), key t of it at slot
+ * page_table[b * max_pages + t / page] * page + t % page, and the queries
+ * cu_q[b] .. cu_q[b + 1] (device int32 [B + 1], ascending; NULL: one query
+ * per sequence), at most max_q of them. Q, O [cu_q[B]][Hq][Dh] of `type`,
+ * contiguous, 16-byte aligned. Query i of n sits at key position
+ * s = kv_len[b] - n + i: causal masks t > s, window > 0 masks
+ * t < s - window + 1. scale <= 0 means 1 / sqrt(Dh). Queries with no key
+ * left give 0; rows of O past cu_q[B] are left as they were. Scores, softmax
+ * and sums in f32; f32 queries keep f32 accuracy (the weights are rounded
+ * to 11 bits for the 16-bit types). Limits: queries beyond max_q in a
+ * sequence are not computed; key positions past max_pages * page, or on a
+ * page number outside the cache, are taken as masked, and the next
+ * rouge_b200_sync_status returns ROUGE_B200_EINVAL. The workspace
+ * (rouge_b200_attention_kv4_workspace bytes, 256-byte aligned, no
+ * initialisation) belongs to the call until it has finished: calls that may
+ * run at the same time, captured graphs among them, each need their own. */
+size_t rouge_b200_attention_kv4_workspace(int B, int Hq, int Hkv, int Dh, int max_q, int max_kv,
+                                          int type);
+int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type, int B, int Hq,
+                             const int *cu_q, int max_q, const int *kv_len, const int *page_table,
+                             int max_pages, void *O, float scale, int causal, int window,
+                             void *workspace, size_t workspace_bytes, void *stream);
 
 /* Convolution forward with cuDNN's semantics (the operation the reference
  * runs in cudnnConvolutionForward, cudnn_shim.cpp:188-232, on its CPU

@@ -1,0 +1,250 @@
+// Writing to and reading from the paged 4-bit key / value cache.
+//
+// One thread per block of 16 values of one token and head: 16 elements in
+// registers, so the block's maximum needs no shuffle, and 8 bytes of codes
+// plus one scale byte out (or the reverse). Neighbouring threads hold
+// neighbouring blocks, so a warp reads whole lines of K or V and writes
+// whole sectors of the page. Memory-bound: 2 or 4 bytes in and 0.5625 bytes
+// out per value.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kv4.cuh"
+#include "narrow.cuh"
+#include "x86fp.cuh"
+
+namespace rb200 {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct KvArgs {
+  uint8_t *codes[2], *scales[2];
+  const float *gs[2];
+  const void *src[2];
+  void *dst[2];
+  long long ld[2];
+  int page, Hkv, nblk;  // nblk = Dh / 16
+  int total_slots;
+  long long items;      // T * Hkv * nblk
+  const int *slots;
+  int *err;
+};
+
+template <int T>
+__device__ __forceinline__ void load16(const void *p, long long at, float (&v)[16]) {
+  if constexpr (T == ROUGE_B200_T_F32) {
+    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 t = __ldg(q + i);
+      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+    }
+  } else {
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
+    const uint4 t0 = __ldg(q), t1 = __ldg(q + 1);
+    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (T == ROUGE_B200_T_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void store16(void *p, long long at, const float (&v)[16]) {
+  if constexpr (T == ROUGE_B200_T_F32) {
+    float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      u[i] = T == ROUGE_B200_T_F16 ? f16x2_rn(v[2 * i], v[2 * i + 1]) : bf16x2_rn(v[2 * i], v[2 * i + 1]);
+    uint4 *q = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at);
+    q[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    q[1] = make_uint4(u[4], u[5], u[6], u[7]);
+  }
+}
+
+// Where item i (token, head, block) lies: false for a skipped token.
+__device__ __forceinline__ bool locate(const KvArgs &a, long long i, int &head, long long &el,
+                                       int which, size_t &blk_at) {
+  const int blk = static_cast<int>(i % a.nblk);
+  const long long th = i / a.nblk;
+  head = static_cast<int>(th % a.Hkv);
+  const long long t = th / a.Hkv;
+  const int slot = __ldg(a.slots + t);
+  if (slot < 0) return false;
+  if (slot >= a.total_slots) {
+    atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
+    return false;
+  }
+  el = t * a.ld[which] + (static_cast<long long>(head) * a.nblk + blk) * 16;
+  const int p = slot / a.page, at = slot - p * a.page;
+  blk_at = ((static_cast<size_t>(p) * a.Hkv + head) * a.page + at) * a.nblk + blk;
+  return true;
+}
+
+// x / step for a code's border test, correctly rounded: one Newton step on
+// the product with the reciprocal, whose residual is exact while nothing
+// under- or overflows (step between 2^-100 and 2^100); a quotient that is
+// exactly a border between two codes is then met exactly.
+__device__ __forceinline__ float quotient(float x, float step, float inv, bool plain) {
+  if (plain) return __fdiv_rn(x, step);
+  const float q = __fmul_rn(x, inv);
+  const float r = __fmaf_rn(-q, step, x);
+  return fabsf(q) < 8.0f ? __fmaf_rn(r, inv, q) : q;  // (6 and more saturate; NaN and Inf stay)
+}
+
+// -0.25 <= v <= 0 codes +0 (the hardware keeps the sign of a zero).
+__device__ __forceinline__ float drop_sign(float v) { return (v >= -0.25f && v <= 0.0f) ? 0.0f : v; }
+
+template <int T>
+__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
+  const int which = blockIdx.y;
+  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < a.items;
+       i += static_cast<long long>(gridDim.x) * kThreads) {
+    int head;
+    long long el;
+    size_t at;
+    if (!locate(a, i, head, el, which, at)) continue;
+    float v[16];
+    load16<T>(a.src[which], el, v);
+    const float g = a.gs[which] ? __ldg(a.gs[which] + head) : 1.0f;
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = fmaxf(m, fabsf(v[j]));
+    const uint32_t sc = cvt_pair_e4m3(__fdiv_rn(m, __fmul_rn(6.0f, g)), 0.0f) & 0xFFu;
+    const uint32_t sh = e4m3x2_f16x2(sc);
+    const float step = __fmul_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(sh))), g);
+    uint2 w = make_uint2(0u, 0u);
+    if (step > 0.0f) {
+      const bool plain = !(step > 7.9e-31f && step < 1.2e30f);
+      const float inv = __fdiv_rn(1.0f, step);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = drop_sign(quotient(v[j], step, inv, plain));
+      w.x = cvt4_e2m1(v[0], v[1], v[2], v[3]) | (cvt4_e2m1(v[4], v[5], v[6], v[7]) << 16);
+      w.y = cvt4_e2m1(v[8], v[9], v[10], v[11]) | (cvt4_e2m1(v[12], v[13], v[14], v[15]) << 16);
+    }
+    reinterpret_cast<uint2 *>(a.codes[which])[at] = w;
+    a.scales[which][at] = static_cast<uint8_t>(sc);
+  }
+}
+
+template <int T>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const KvArgs a) {
+  const int which = blockIdx.y;
+  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < a.items;
+       i += static_cast<long long>(gridDim.x) * kThreads) {
+    int head;
+    long long el;
+    size_t at;
+    if (!locate(a, i, head, el, which, at)) continue;
+    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(a.codes[which]) + at);
+    const uint32_t sh = e4m3x2_f16x2(__ldg(a.scales[which] + at));
+    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sh)));
+    const float g = a.gs[which] ? __ldg(a.gs[which] + head) : 1.0f;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t h[4];
+      e2m1x8_f16x2(k ? w.y : w.x, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+        v[8 * k + 2 * j] = __fmul_rn(__fmul_rn(f.x, s), g);  // (code * scale is exact)
+        v[8 * k + 2 * j + 1] = __fmul_rn(__fmul_rn(f.y, s), g);
+      }
+    }
+    store16<T>(a.dst[which], el, v);
+  }
+}
+
+int prepare(const RougeB200KV4 *c, const void *K, long long ldk, const void *V, long long ldv,
+            int type, int T, const int *slots, KvArgs &a) {
+  int s = check_kv4(c);
+  if (s != ROUGE_B200_OK) return s;
+  if (T < 0 || !valid_float_type(type)) return ROUGE_B200_EINVAL;
+  if (T == 0) return ROUGE_B200_OK;
+  const long long row = static_cast<long long>(c->Hkv) * c->Dh;
+  if (!K || !V || !slots || ldk < row || ldv < row) return ROUGE_B200_EINVAL;
+  const int es = type == ROUGE_B200_T_F32 ? 4 : 2;
+  if (((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V)) & 15u) ||
+      (ldk * es) % 16 || (ldv * es) % 16 || (reinterpret_cast<uintptr_t>(slots) & 3u))
+    return ROUGE_B200_EUNSUPPORTED;
+  a.codes[0] = c->k_codes; a.codes[1] = c->v_codes;
+  a.scales[0] = c->k_scales; a.scales[1] = c->v_scales;
+  a.gs[0] = c->gs_k; a.gs[1] = c->gs_v;
+  a.ld[0] = ldk; a.ld[1] = ldv;
+  a.page = c->page;
+  a.Hkv = c->Hkv;
+  a.nblk = c->Dh / 16;
+  a.total_slots = c->pages * c->page;
+  a.items = static_cast<long long>(T) * c->Hkv * a.nblk;
+  a.slots = slots;
+  return ROUGE_B200_OK;
+}
+
+dim3 grid_of(const KvArgs &a) {
+  const long long want = (a.items + kThreads - 1) / kThreads;
+  const long long cap = static_cast<long long>(current_sm_count()) * 8;
+  return dim3(static_cast<unsigned>(want < cap ? want : cap), 2);
+}
+
+}  // namespace
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" {
+
+int rouge_b200_kv4_write(const RougeB200KV4 *cache, const void *K, long long ldk, const void *V,
+                         long long ldv, int type, int T, const int *slots, void *stream) {
+  KvArgs a{};
+  int s = prepare(cache, K, ldk, V, ldv, type, T, slots, a);
+  if (s != ROUGE_B200_OK) return set_status(s);
+  s = device_ready();
+  if (s != ROUGE_B200_OK || T == 0) return s;
+  a.src[0] = K;
+  a.src[1] = V;
+  a.err = device_error_word();
+  if (!a.err) return set_status(ROUGE_B200_ENOMEM);
+  cudaStream_t st = as_stream(stream);
+  switch (type) {
+    case ROUGE_B200_T_F32: kv4_write_kernel<ROUGE_B200_T_F32><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    case ROUGE_B200_T_F16: kv4_write_kernel<ROUGE_B200_T_F16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    default: kv4_write_kernel<ROUGE_B200_T_BF16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+  }
+  return cuda_status(cudaGetLastError());
+}
+
+int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void *V, long long ldv,
+                        int type, int T, const int *slots, void *stream) {
+  KvArgs a{};
+  int s = prepare(cache, K, ldk, V, ldv, type, T, slots, a);
+  if (s != ROUGE_B200_OK) return set_status(s);
+  s = device_ready();
+  if (s != ROUGE_B200_OK || T == 0) return s;
+  a.dst[0] = K;
+  a.dst[1] = V;
+  a.err = device_error_word();
+  if (!a.err) return set_status(ROUGE_B200_ENOMEM);
+  cudaStream_t st = as_stream(stream);
+  switch (type) {
+    case ROUGE_B200_T_F32: kv4_read_kernel<ROUGE_B200_T_F32><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    case ROUGE_B200_T_F16: kv4_read_kernel<ROUGE_B200_T_F16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    default: kv4_read_kernel<ROUGE_B200_T_BF16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+  }
+  return cuda_status(cudaGetLastError());
+}
+
+}  // extern "C"

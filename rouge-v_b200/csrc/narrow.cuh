@@ -17,6 +17,9 @@
 #include <cstdint>
 
 #include "formats.cuh"
+#if defined(__CUDACC__)
+#include "x86fp.cuh"
+#endif
 
 namespace rb200 {
 
@@ -173,6 +176,42 @@ __device__ __forceinline__ uint32_t encode_e2m1(float v) {
                      (a >= 3.5f) + (a > 5.0f);
   const uint32_t s = (a >= 0.25f || a == 0.0f) ? (__float_as_uint(v) >> 31) << 3 : 0u;
   return s | c;
+}
+
+// e4m3 / e5m2 codes of x * inv for an MX block (inv = 2^(127 - scale code),
+// so every finite |x * inv| <= emax / 2: the reference's overflow edges are
+// out of reach). The hardware conversion equals the reference except for
+// NaN (sign kept by the reference) and for nonzero magnitudes below half
+// the smallest subnormal, which the hardware rounds to a signed zero and
+// the reference to +0. Both show cheaply per group of four: a NaN makes
+// the sum NaN, a signed zero is a 0x80 byte; such groups take the exact
+// path (x86 products, the reference encoder).
+template <int ID>
+__device__ __forceinline__ uint32_t mx_encode4_f8(float4 x, float inv) {
+  const float sum = (x.x + x.y) + (x.z + x.w);
+  const uint32_t lo = ID == kE4M3 ? cvt_pair_e4m3(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv))
+                                  : cvt_pair_e5m2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
+  const uint32_t hi = ID == kE4M3 ? cvt_pair_e4m3(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv))
+                                  : cvt_pair_e5m2(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
+  const uint32_t w = lo | (hi << 16);
+  if (sum == sum && __vcmpeq4(w, 0x80808080u) == 0u) return w;
+  return narrow_encode(x86_mul(x.x, inv), ID, false) |
+         (narrow_encode(x86_mul(x.y, inv), ID, false) << 8) |
+         (narrow_encode(x86_mul(x.z, inv), ID, false) << 16) |
+         (narrow_encode(x86_mul(x.w, inv), ID, false) << 24);
+}
+
+// Four e2m1 codes (RNE, satfinite) from the hardware conversion, one per
+// nibble, x0 in the low nibble.
+__device__ __forceinline__ uint32_t cvt4_e2m1(float x0, float x1, float x2, float x3) {
+  uint16_t r;
+  asm("{\n\t.reg .b8 t0, t1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
+      "mov.b16 %0, {t0, t1};\n\t}"
+      : "=h"(r)
+      : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+  return r;
 }
 #endif
 

@@ -71,6 +71,19 @@ class GemmProfile(C.Structure):
     """RougeGemmProfile (numerics.h:44-48)."""
     _fields_ = [("cfg", GemmConfig), ("gflops", C.c_double), ("iters", C.c_longlong)]
 
+
+class _EpilogueC(C.Structure):
+    """RougeB200Epilogue."""
+    _fields_ = [("bias", _P), ("residual", _P), ("ldr", C.c_longlong), ("residual_type", _I), ("act", _I)]
+
+
+class _KV4C(C.Structure):
+    """RougeB200KV4."""
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("gs_k", _P),
+                ("gs_v", _P), ("pages", _I), ("page", _I), ("Hkv", _I), ("Dh", _I)]
+
+
+_LL = C.c_longlong
 _SIGS = {
     "rouge_b200_last_error": (_I, []),
     "rouge_b200_clear_error": (None, []),
@@ -133,6 +146,12 @@ _SIGS = {
     "rouge_b200_transformer_block_workspace": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "rouge_b200_transformer_block": (_I, [_I] * 6 + [_P] * 10 + [_I, C.c_float, C.c_float, _P, _P,
                                                                   _SZ, _P]),
+    "rouge_b200_add_rmsnorm_quant": (_I, [_P, _LL, _P, _LL, _P, _F, _I, _I, _I, _P, _LL, _I, _P, _P, _P]),
+    "rouge_b200_kv4_write": (_I, [C.POINTER(_KV4C), _P, _LL, _P, _LL, _I, _I, _P, _P]),
+    "rouge_b200_kv4_read": (_I, [C.POINTER(_KV4C), _P, _LL, _P, _LL, _I, _I, _P, _P]),
+    "rouge_b200_attention_kv4_workspace": (_SZ, [_I] * 7),
+    "rouge_b200_attention_kv4": (_I, [C.POINTER(_KV4C), _P, _I, _I, _I, _P, _I, _P, _P, _I, _P, _F, _I, _I,
+                                      _P, _SZ, _P]),
     "rouge_b200_mxfp4_scale_atoms_bytes": (_SZ, [_I, _I]),
     "rouge_b200_mxfp4_scale_atoms": (_I, [_P, _I, _I, _P, _P]),
     "rouge_b200_gemm_mxfp4": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P]),
@@ -153,6 +172,12 @@ _SIGS = {
                                       C.c_longlong, _I, _I, _P]),
     "rouge_b200_gemm_e4m3": (_I, [_I, _I, _I, _P, _P, _I, _P, _P, _P, _I, _I, _P]),
     "rouge_b200_gemm_f16": (_I, [_I, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P]),
+    "rouge_b200_gemm_i8_fused": (_I, [_I, _I, _I, _P, _P, _I, _P, _I, _P, _I, C.POINTER(_EpilogueC),
+                                      _P, _I, _I, _P]),
+    "rouge_b200_gemm_e4m3_fused": (_I, [_I, _I, _I, _P, _P, _I, _P, _P, C.POINTER(_EpilogueC), _P, _I,
+                                        _I, _P]),
+    "rouge_b200_gemm_f16_fused": (_I, [_I, _I, _I, _P, _P, _I, _I, C.POINTER(_EpilogueC), _P, _I, _I,
+                                       _P]),
     "rouge_b200_conv2d_nhwc_f16": (_I, [_I] * 9 + [_P, _P, _P, _P, _I, _P]),
     "rouge_b200_synth_uniform": (_I, [_U64, _SZ, _F, _F, _P]),
     "rouge_b200_synth_normal": (_I, [_U64, _SZ, _F, _F, _P]),
@@ -373,6 +398,114 @@ def transformer_block(x, wrms1, wq, wk, wv, wo, wrms2, wgate, wup, wdown, Hq, Hk
         workspace.numel(), _stream()))
 
 
+Q_I8_ROWS, Q_MX_E4M3 = 0, 1
+
+
+def add_rmsnorm_quant(x, residual, w, eps, out_fmt, codes, scales, h_out=None):
+    """h_out = x + residual (both None: h = x), then the 8-bit codes and scales of
+    RMSNorm(h) * w: out_fmt Q_I8_ROWS (int8 [rows][cols], f32 [rows]) or Q_MX_E4M3
+    (uint8 [rows][cols], uint8 [rows][cols / 32]). Rows of x, residual and h_out
+    may be strided; codes and scales are contiguous."""
+    rows, cols = x.shape
+    for t in (residual, h_out):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("residual and h_out: shape and type of x expected")
+    for t in (x, residual, h_out):
+        if t is not None and cols > 1 and t.stride(1) != 1:
+            raise ValueError("contiguous rows expected")
+    ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else max(cols, t.stride(0))  # noqa: E731
+    _check("rouge_b200_add_rmsnorm_quant", lib().rouge_b200_add_rmsnorm_quant(
+        _dp(x), ld(x), _dp(residual), ld(residual), _dp(w), eps, rows, cols, _type_of(x), _dp(h_out),
+        ld(h_out), out_fmt, _dp(codes), _dp(scales), _stream()))
+
+
+class KV4Cache:
+    """A paged 4-bit key / value cache (RougeB200KV4): uint8 tensors
+    k_codes, v_codes [pages][Hkv][page][Dh / 2], k_scales, v_scales
+    [pages][Hkv][page][Dh / 16] (contiguous), gs_k, gs_v f32 [Hkv] or None."""
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales, gs_k=None, gs_v=None):
+        pages, Hkv, page, half = k_codes.shape
+        codes, scales = (pages, Hkv, page, half), (pages, Hkv, page, half // 8)
+        for t, shape in ((k_codes, codes), (k_scales, scales), (v_codes, codes), (v_scales, scales)):
+            if t.shape != shape or t.element_size() != 1 or not t.is_contiguous():
+                raise ValueError(f"contiguous bytes {shape} expected, got {tuple(t.shape)}")
+        for t in (gs_k, gs_v):
+            if t is not None and (t.shape != (Hkv,) or t.element_size() != 4 or not t.is_contiguous()):
+                raise ValueError(f"contiguous float32 [{Hkv}] expected")
+        self.tensors = (k_codes, k_scales, v_codes, v_scales, gs_k, gs_v)
+        self.pages, self.Hkv, self.page, self.Dh = pages, Hkv, page, 2 * half
+        self.c = _KV4C(*(None if t is None else t.data_ptr() for t in self.tensors), pages, page, Hkv,
+                       2 * half)
+
+    @classmethod
+    def empty(cls, pages, Hkv, page, Dh, gs_k=None, gs_v=None, device="cuda"):
+        """A cache of zeros."""
+        import torch
+        z = lambda n: torch.zeros(pages, Hkv, page, n, dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(z(Dh // 2), z(Dh // 16), z(Dh // 2), z(Dh // 16), gs_k, gs_v)
+
+
+def _kv4_tokens(cache, K, V, slots):
+    import torch
+    T = K.shape[0]
+    for t in (K, V):
+        if t.shape != (T, cache.Hkv, cache.Dh) or t.dtype != K.dtype or (T and (
+                t.stride(2) != 1 or t.stride(1) != cache.Dh)):
+            raise ValueError(f"[{T}, {cache.Hkv}, {cache.Dh}] with contiguous tokens expected")
+    if slots.shape != (T,) or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise ValueError(f"slots: contiguous int32 [{T}] expected")
+    ld = lambda t: max(t.stride(0), cache.Hkv * cache.Dh) if T < 2 else t.stride(0)  # noqa: E731
+    return (_dp(K), ld(K), _dp(V), ld(V), _type_of(K), T, _dp(slots), _stream())
+
+
+def kv4_write(cache, K, V, slots):
+    """K, V [T][Hkv][Dh] (f32, f16 or bf16; tokens may be strided) into the
+    slots [T] (int32; negative: skipped) of a KV4Cache."""
+    _check("rouge_b200_kv4_write",
+           lib().rouge_b200_kv4_write(C.byref(cache.c), *_kv4_tokens(cache, K, V, slots)))
+
+
+def kv4_read(cache, slots, K, V):
+    """The values of slots [T] into K, V [T][Hkv][Dh]."""
+    _check("rouge_b200_kv4_read",
+           lib().rouge_b200_kv4_read(C.byref(cache.c), *_kv4_tokens(cache, K, V, slots)))
+
+
+def attention_kv4_workspace(B, Hq, Hkv, Dh, max_q, max_kv, type):
+    return lib().rouge_b200_attention_kv4_workspace(B, Hq, Hkv, Dh, max_q, max_kv, type)
+
+
+def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scale=0.0, causal=1,
+                  window=0, workspace=None):
+    """O[T][Hq][Dh] of Q[T][Hq][Dh] over a KV4Cache: sequence b has kv_len[b] keys
+    on the pages page_table[b] and the queries cu_q[b] .. cu_q[b + 1] (None: one
+    each). workspace: uint8, attention_kv4_workspace() bytes."""
+    import torch
+    B, max_pages = page_table.shape
+    T, Hq, Dh = Q.shape
+    if O is None:
+        O = torch.empty_like(Q)
+    if O.shape != Q.shape or O.dtype != Q.dtype or not O.is_contiguous() or not Q.is_contiguous():
+        raise ValueError("Q, O: contiguous, of one shape and type")
+    if Dh != cache.Dh:
+        raise ValueError(f"head size {Dh}, and {cache.Dh} in the cache")
+    for t, shape in ((kv_len, (B,)), (page_table, (B, max_pages)), (cu_q, (B + 1,))):
+        if t is not None and (t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous()):
+            raise ValueError(f"contiguous int32 {shape} expected")
+    if cu_q is None and (T < B or max_q != 1):
+        raise ValueError("without cu_q: one query per sequence")
+    ty = _type_of(Q)
+    if workspace is None:
+        workspace = torch.empty(attention_kv4_workspace(B, Hq, cache.Hkv, Dh, max_q,
+                                                        max_pages * cache.page, ty),
+                                dtype=torch.uint8, device=Q.device)
+    _check("rouge_b200_attention_kv4", lib().rouge_b200_attention_kv4(
+        C.byref(cache.c), _dp(Q), ty, B, Hq, _dp(cu_q), max_q, _dp(kv_len), _dp(page_table), max_pages,
+        _dp(O), scale, causal, window, _dp(workspace), workspace.numel(), _stream()))
+    return O
+
+
 def convert_f32_to_f16(x, out):
     _check("rouge_b200_convert_f32_to_f16", lib().rouge_b200_convert_f32_to_f16(
         _dp(x), x.numel(), _dp(out), _stream()))
@@ -388,9 +521,52 @@ def convert_e4m3_to_f32(x, out):
         _dp(x), x.numel(), _dp(out), _stream()))
 
 
-def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None, b_cols=1):
+T_F32, T_F16, T_BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+
+
+def _type_of(t):
+    """ROUGE_B200_T_* of a floating tensor."""
+    import torch
+    types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
+    if t.dtype not in types:
+        raise TypeError(f"float32, float16 or bfloat16 tensor expected, got {t.dtype}")
+    return types[t.dtype]
+
+
+class Epilogue:
+    """Epilogue of gemm_i8 / gemm_e4m3 / gemm_f16: act(. + bias[n]) + residual[m][n],
+    each optional. bias: f32 [N]; residual: f32, f16 or bf16 [M][N], rows
+    contiguous (it may be the output tensor itself); act: ACT_*."""
+
+    def __init__(self, bias=None, act=ACT_NONE, residual=None):
+        self.tensors = (bias, residual)  # (kept alive)
+        self.c = _EpilogueC(None if bias is None else bias.data_ptr(),
+                            None if residual is None else residual.data_ptr(),
+                            0 if residual is None else residual.stride(0),
+                            T_F32 if residual is None else _type_of(residual), act)
+
+    def check(self, M, N):
+        """Raises unless the tensors fit an M x N output."""
+        import torch
+        bias, residual = self.tensors
+        if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or
+                                 not bias.is_contiguous()):
+            raise ValueError(f"bias: contiguous float32 [{N}] expected")
+        if residual is not None and (residual.shape != (M, N) or (N > 1 and residual.stride(1) != 1)):
+            raise ValueError(f"residual: [{M}, {N}] with contiguous rows expected")
+
+
+def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None, b_cols=1,
+            epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
+    if epilogue is not None:
+        epilogue.check(M, N)
+        _check("rouge_b200_gemm_i8_fused", lib().rouge_b200_gemm_i8_fused(
+            M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
+            C.byref(epilogue.c), _dp(C_), C_.stride(0), out_type, _stream()))
+        return
     _check("rouge_b200_gemm_i8", lib().rouge_b200_gemm_i8(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
         _dp(C_), C_.stride(0), out_type, _stream()))
@@ -428,17 +604,29 @@ def w8a8_linear(X, Wq, sw, Aq, sa, C_, out_type, ws):
         _dp(ws), _stream()))
 
 
-def gemm_e4m3(A, B, b_layout, C_, out_type, scale_a=None, scale_b=None):
+def gemm_e4m3(A, B, b_layout, C_, out_type, scale_a=None, scale_b=None, epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
+    if epilogue is not None:
+        epilogue.check(M, N)
+        _check("rouge_b200_gemm_e4m3_fused", lib().rouge_b200_gemm_e4m3_fused(
+            M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), C.byref(epilogue.c),
+            _dp(C_), C_.stride(0), out_type, _stream()))
+        return
     _check("rouge_b200_gemm_e4m3", lib().rouge_b200_gemm_e4m3(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), _dp(C_), C_.stride(0),
         out_type, _stream()))
 
 
-def gemm_f16(A, B, b_layout, C_, out_type, is_bf16=False):
+def gemm_f16(A, B, b_layout, C_, out_type, is_bf16=False, epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
+    if epilogue is not None:
+        epilogue.check(M, N)
+        _check("rouge_b200_gemm_f16_fused", lib().rouge_b200_gemm_f16_fused(
+            M, N, K, _dp(A), _dp(B), b_layout, int(is_bf16), C.byref(epilogue.c), _dp(C_),
+            C_.stride(0), out_type, _stream()))
+        return
     _check("rouge_b200_gemm_f16", lib().rouge_b200_gemm_f16(
         M, N, K, _dp(A), _dp(B), b_layout, int(is_bf16), _dp(C_), C_.stride(0), out_type,
         _stream()))

@@ -1,0 +1,441 @@
+"""The paged 4-bit cache and the attention over it against 64-bit arithmetic.
+
+Written codes and scales: equal to the definition (quotients exact in 64 bits
+at every tie a 16-bit input can meet). Read values: one rounding to the type.
+
+Attention: with Q and the cache exact, a score's error is that of its f32
+accumulation, at most (Dh / 16 + 6) roundings of 2^-23 of the sum of |q k| --
+call it ds --, each weight is off by a factor within 2 ds, the exponential's
+2^-21 and, for the 16-bit types, the 2^-11 of an f16 weight (f32 queries
+split it: 2^-21); the weighted sums add one 2^-23 per 16 keys of a warp's run
+and per joined part. So |O - exact| <= (2 ds + w + n 2^-23) sum_t p_t |v_t|,
+plus half a step of the output's type. Below the normal f16 range a weight is off
+by half a subnormal step instead: the kernel holds 2^15 exp(s - max) in f16, whose
+subnormal step is 2^-24, so a weight relative to the largest one is off by at
+most 2^-25 / 2^15 = 2^-40, and O (divided by a sum of at least 1) by
+2^-40 sum_t |v_t|. (It shows where the heavy keys hold zeros in a column.) The
+output's half step is eps / 2 of the value, or half the subnormal step, which is
+smallest_normal * eps / 2, for values that f16 holds as subnormals."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+E2M1 = [0, 0.5, 1, 1.5, 2, 3, 4, 6]
+
+
+def _dt(t):
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[t]
+
+
+def _half_step(v, dtype):
+    import torch
+    f = torch.finfo(dtype)
+    return v.clamp(min=f.smallest_normal) * f.eps / 2
+
+
+def _lut():
+    import torch
+    return torch.tensor(E2M1 + [-v for v in E2M1], dtype=torch.float64, device="cuda")
+
+
+def _decode(codes, scales, gs):
+    """[pages][Hkv][page][Dh] in 64 bits."""
+    import torch
+    c = codes.long()
+    v = torch.stack((c & 15, c >> 4), -1).flatten(-2)
+    s = scales.view(torch.float8_e4m3fn).double().repeat_interleave(16, -1)
+    return _lut()[v] * s * gs.double()[None, :, None, None]
+
+
+def _quantize(x, g):
+    """Codes and e4m3 scales of x [..., Dh] by the definition; g broadcast over blocks."""
+    import torch
+    b = x.double().unflatten(-1, (-1, 16))
+    m = b.abs().nan_to_num(0, posinf=math.inf).amax(-1)
+    s = (m.float() / (6 * g)).clamp(max=448).to(torch.float8_e4m3fn)
+    step = (s.double() * g.double())[..., None]
+    z = torch.where(step > 0, b / step, torch.zeros_like(b))
+    grid = _lut()[:8]
+    mid = (grid[1:] + grid[:-1]) / 2
+    k = torch.bucketize(z.abs(), mid)
+    k = torch.where((k < 7) & (k % 2 == 1) & (z.abs() == mid[k.clamp(max=6)]), k + 1, k)
+    k = torch.where(z.isnan(), torch.full_like(k, 7), k + 8 * ((z < 0) & (k > 0)))
+    k = k.flatten(-2)
+    return (k[..., 0::2] | (k[..., 1::2] << 4)).to(torch.uint8), s.view(torch.uint8)
+
+
+def _cache(rb, pages, Hkv, page, Dh, seed, gs=True):
+    """A cache of random codes, its scales between 2^-3 and 2; slots nothing wrote are poisoned by the tests."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(seed)
+    by = lambda n: torch.randint(0, 256, (pages, Hkv, page, n), generator=g, device="cuda").to(torch.uint8)  # noqa: E731
+    sc = lambda: torch.randint(32, 65, (pages, Hkv, page, Dh // 16), generator=g, device="cuda").to(torch.uint8)  # noqa: E731
+    gg = lambda: (0.3 + torch.rand(Hkv, generator=g, device="cuda")) if gs else None  # noqa: E731
+    return rb.KV4Cache(by(Dh // 2), sc(), by(Dh // 2), sc(), gg(), gg())
+
+
+def _reference(cache, q, lens, table, nqs, causal, window, scale):
+    """O and the tolerance's parts in 64 bits, sequence by sequence."""
+    import torch
+    kc, ks, vc, vs, gk, gv = cache.tensors
+    one = torch.ones(cache.Hkv, device="cuda")
+    K, V = _decode(kc, ks, gk if gk is not None else one), _decode(vc, vs, gv if gv is not None else one)
+    Hq = q.shape[1]
+    G = Hq // cache.Hkv
+    out, spread, ds, tiny = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(4))
+    at = 0
+    for b, (n, nq) in enumerate(zip(lens, nqs)):
+        for i in range(nq):
+            p = n - nq + i
+            hi = max(0, min(n, p + 1)) if causal else n
+            lo = max(0, p - window + 1) if window else 0
+            if hi > lo:
+                t = torch.arange(lo, hi, device="cuda")
+                pg, off = table[b].long()[t // cache.page], t % cache.page
+                k = K[pg, :, off].repeat_interleave(G, 1)
+                v = V[pg, :, off].repeat_interleave(G, 1)
+                z = torch.einsum("hd,thd->ht", q[at].double(), k) * scale
+                za = torch.einsum("hd,thd->ht", q[at].double().abs(), k.abs()) * scale
+                w = torch.softmax(z, 1)
+                out[at] = torch.einsum("ht,thd->hd", w, v)
+                spread[at] = torch.einsum("ht,thd->hd", w, v.abs())
+                tiny[at] = 2.0 ** -40 * v.abs().sum(0)
+                ds[at] = (za.amax(1) * (cache.Dh / 16 + 6) * 2.0 ** -23)[:, None]
+            at += 1
+    return out, spread, ds, tiny
+
+
+def _attend(rb, cache, t, lens, nqs, Hq, causal=1, window=0, scale=0.0, seed=0, extra=0, table=None):
+    import torch
+    g = torch.Generator("cuda").manual_seed(seed)
+    per = max(1, max(-(-n // cache.page) for n in lens))
+    if table is None:
+        order = torch.randperm(cache.pages, generator=g, device="cuda").int()
+        table = torch.full((len(lens), per), 1 << 30, dtype=torch.int32, device="cuda")  # (never read past a length)
+        at = 0
+        for b, n in enumerate(lens):
+            k = -(-n // cache.page)
+            table[b, :k] = order[at:at + k]
+            at += k
+    T = sum(nqs)
+    q = torch.randn(T + extra, Hq, cache.Dh, generator=g, device="cuda").to(_dt(t))
+    O = torch.full_like(q, 77.0)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu = torch.tensor(np.concatenate(([0], np.cumsum(nqs))), dtype=torch.int32, device="cuda")
+    single = all(n == 1 for n in nqs)
+    rb.attention_kv4(q, cache, lens_d, table, cu_q=None if single else cu, max_q=1 if single else max(max(nqs), 1),
+                     O=O, scale=scale, causal=causal, window=window)
+    return q, O, table, lens_d, cu
+
+
+def _check(rb, cache, t, lens, nqs, Hq, causal=1, window=0, scale=0.0, **kw):
+    import torch
+    q, O, table, _, _ = _attend(rb, cache, t, lens, nqs, Hq, causal, window, scale, **kw)
+    rb.sync_status()
+    T = sum(nqs)
+    want, spread, ds, tiny = _reference(cache, q, lens, table, nqs, causal, window, scale or 1 / math.sqrt(cache.Dh))
+    w = 2.0 ** -21 + (2.0 ** -21 if t == "f32" else 2.0 ** -11)
+    n = max(max(lens), 16) / 16 + 64
+    tol = (2 * ds + w + n * 2.0 ** -23) * spread + tiny
+    tol = tol + _half_step(want.abs() + tol, q.dtype)
+    d = (O[:T].double() - want[:T]).abs()
+    assert (d <= tol[:T]).all(), ((d / tol[:T].clamp(min=1e-300)).nan_to_num(math.inf).max().item(), d.max().item())
+    assert (O[T:] == 77).all()
+    return O
+
+
+# ------------------------------------------------------------------ write, read
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,Hkv,Dh,page,gs", [(1, 1, 16, 16, False), (5, 2, 64, 16, True), (70, 3, 80, 48, True),
+                                              (300, 8, 128, 64, True), (33, 1, 256, 32, False)])
+def test_write_and_read(rb, cuda, t, T, Hkv, Dh, page, gs):
+    import torch
+    g = torch.Generator("cuda").manual_seed(T)
+    pages = -(-T // page) + 2
+    gk, gv = ((0.25 * 2.0 ** torch.randint(0, 4, (Hkv,), generator=g, device="cuda")).float() for _ in range(2))
+    cache = rb.KV4Cache.empty(pages, Hkv, page, Dh, gk if gs else None, gv if gs else None)
+    one = torch.ones(Hkv, device="cuda")
+    gk, gv = (gk, gv) if gs else (one, one)
+    big = torch.randn(T, 2, Hkv, Dh, generator=g, device="cuda") * torch.exp(
+        3 * torch.randn(T, 2, Hkv, 1, generator=g, device="cuda"))
+    big[0, 0, 0, :16] = 0  # an empty block
+    big = big.to(_dt(t))
+    K, V = big[:, 0], big[:, 1]  # (strided tokens)
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:T].int()
+    if T > 4:
+        slots[2] = -1
+    rb.kv4_write(cache, K, V, slots)
+    rb.sync_status()
+    keep = slots >= 0
+    pg, at = slots[keep].long() // page, slots[keep].long() % page
+    used = torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+    used[pg, at] = True
+    k2, v2 = torch.full_like(K, 9).contiguous(), torch.full_like(V, 9).contiguous()
+    rb.kv4_read(cache, slots, k2, v2)
+    rb.sync_status()
+    for x, codes, scales, gg, back in ((K, cache.tensors[0], cache.tensors[1], gk, k2),
+                                       (V, cache.tensors[2], cache.tensors[3], gv, v2)):
+        c, s = _quantize(x[keep], gg[None, :, None])
+        assert torch.equal(codes[pg, :, at], c) and torch.equal(scales[pg, :, at], s)
+        assert (codes.transpose(1, 2)[~used] == 0).all() and (scales.transpose(1, 2)[~used] == 0).all()
+        want = _decode(codes, scales, gg)[pg, :, at]
+        assert torch.equal(back[keep], want.float().to(_dt(t)))
+        assert (back[~keep] == 9).all()
+
+
+def test_write_ties_and_specials(rb, cuda):
+    """Every border between two codes, saturation, signed zeros, NaN and infinities, subnormal and huge scales."""
+    import torch
+    cache = rb.KV4Cache.empty(2, 1, 16, 64)
+    K = torch.zeros(6, 1, 64, device="cuda")
+    K[0, 0, :16] = torch.tensor([6, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, -.25, -.75, -1.25, -1.75, -2.5, -3.5, -5, -.2])
+    K[0, 0, 16:32] = 3 * K[0, 0, :16]
+    K[1, 0, :16] = torch.tensor([float("nan"), 1, -1, 0.5, 2, -6] + [0.0] * 10)
+    K[2, 0, :16] = torch.tensor([float("inf"), -float("inf"), 448 * 6, 448 * 3, -448, 1] + [-0.0] * 10)
+    K[3, 0, :16] = 1e-4 * torch.arange(16)   # a subnormal e4m3 scale
+    K[4, 0, :16] = 1e30
+    K[4, 0, 16:32] = 1e-6                    # rounds to a zero scale
+    K[5, 0, :] = float("nan")
+    for t in ("f32", "bf16"):
+        x = K.to(_dt(t))
+        rb.kv4_write(cache, x, x, torch.arange(6, dtype=torch.int32, device="cuda"))
+        rb.sync_status()
+        c, s = _quantize(x, torch.ones(1, 1, 1, device="cuda"))
+        got = cache.tensors[0][0, 0, :6], cache.tensors[1][0, 0, :6]
+        assert torch.equal(got[1], s[:, 0])
+        live = torch.tensor([0, 1, 2, 3, 4], device="cuda")  # (row 5: no scale, zero codes)
+        assert torch.equal(got[0][live], c[live, 0])
+        assert (got[0][5] == 0).all() and (got[1][5] == 0).all()
+
+
+def test_bad_slots_are_reported(rb, cuda):
+    import torch
+    cache = rb.KV4Cache.empty(2, 2, 16, 32)
+    K = torch.ones(3, 2, 32, device="cuda")
+    slots = torch.tensor([0, 32, 2147483647], dtype=torch.int32, device="cuda")
+    rb.kv4_write(cache, K, K, slots)
+    with pytest.raises(rb.RougeB200Error) as e:
+        rb.sync_status()
+    assert e.value.status == rb.EINVAL
+    assert (cache.tensors[1].transpose(1, 2).reshape(32, -1)[0] != 0).all()
+    assert (cache.tensors[1].transpose(1, 2).reshape(32, -1)[1:] == 0).all()
+    back = torch.full_like(K, 5)
+    rb.kv4_read(cache, slots, back, back.clone())
+    with pytest.raises(rb.RougeB200Error):
+        rb.sync_status()
+    # 1/6 rounds to the e4m3 value 11/64, and 1 / (11/64) = 5.8 to the code of 6
+    assert (back[1:] == 5).all() and (back[0] == 66 / 64).all()
+    rb.kv4_write(cache, K[:0], K[:0], slots[:0])
+    rb.sync_status()
+
+
+# ------------------------------------------------------------------ attention
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Hq,Hkv,Dh,page", [(4, 1, 16, 16), (8, 2, 48, 32), (8, 8, 64, 16), (14, 2, 80, 48),
+                                            (6, 2, 96, 16), (8, 1, 128, 64), (16, 1, 128, 16), (40, 2, 112, 32),
+                                            (4, 2, 192, 16), (9, 1, 256, 128)])
+def test_decode(rb, cuda, t, Hq, Hkv, Dh, page):
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 64, 100, 257, 0]
+    cache = _cache(rb, sum(-(-n // page) for n in lens) + 1, Hkv, page, Dh, Hq + Dh)
+    O = _check(rb, cache, t, lens, [1] * len(lens), Hq)
+    assert (O[-1] == 0).all()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,Hq,Hkv,Dh", [([3000], 8, 1, 128), ([1, 5000, 40, 1023], 8, 2, 64), ([70001], 4, 1, 128),
+                                            ([2049, 2048, 2047], 12, 3, 256)])
+def test_long_sequences_are_split_and_joined(rb, cuda, t, lens, Hq, Hkv, Dh):
+    cache = _cache(rb, sum(-(-n // 64) for n in lens) + 1, Hkv, 64, Dh, 3)
+    _check(rb, cache, t, lens, [1] * len(lens), Hq)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("window", [0, 1, 7, 100])
+def test_queries_and_windows(rb, cuda, t, causal, window):
+    """Ragged numbers of queries: none, one, many, more than keys (those before the first key are empty rows)."""
+    lens, nqs = [40, 5, 200, 33, 0, 130], [3, 9, 1, 33, 2, 0]
+    for Hq, Hkv, Dh in ((6, 2, 64), (5, 1, 80)):
+        cache = _cache(rb, 40, Hkv, 16, Dh, window)
+        _check(rb, cache, t, lens, nqs, Hq, causal, window, extra=3)
+
+
+@pytest.mark.parametrize("nq,n", [(17, 17), (64, 300), (150, 151), (129, 129)])
+@pytest.mark.parametrize("t,Hq,Hkv,Dh", [("bf16", 8, 2, 128), ("f16", 3, 1, 64), ("f32", 4, 4, 64), ("bf16", 2, 1, 256)])
+def test_prompt_chunks(rb, cuda, nq, n, t, Hq, Hkv, Dh):
+    cache = _cache(rb, 2 * (-(-n // 32)) + 2, Hkv, 32, Dh, nq, gs=False)
+    _check(rb, cache, t, [n, n - 1 if n > nq else n], [nq, nq], Hq)
+    _check(rb, cache, t, [n], [nq], Hq, window=20)
+
+
+def test_scale_argument_and_wide_values(rb, cuda):
+    """Queries whose rows differ by 2^40 and a large scale: the row's power of two keeps f16 operands in range."""
+    import torch
+    cache = _cache(rb, 20, 2, 16, 64, 8)
+    g = torch.Generator("cuda").manual_seed(1)
+    lens = torch.tensor([250, 30], dtype=torch.int32, device="cuda")
+    table = torch.arange(32, dtype=torch.int32, device="cuda").reshape(2, 16) % 20
+    q = torch.randn(2, 4, 64, generator=g, device="cuda") * torch.tensor([1e-12, 1e-3, 1.0, 1e5], device="cuda")[:, None]
+    for t in ("f32", "bf16"):
+        qq = q.to(_dt(t))
+        O = rb.attention_kv4(qq, cache, lens, table, scale=1e-5)
+        rb.sync_status()
+        want, spread, ds, tiny = _reference(cache, qq, [250, 30], table, [1, 1], 1, 0, 1e-5)
+        w = 2.0 ** -21 + (2.0 ** -21 if t == "f32" else 2.0 ** -11)
+        tol = (2 * ds + w + 80 * 2.0 ** -23) * spread + tiny
+        tol = tol + _half_step(want.abs() + tol, qq.dtype)
+        assert ((O.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_what_is_masked_is_not_read_into_results(rb, cuda, t):
+    """NaN scales in every slot that no query may see: past the length, before the window, in unused pages."""
+    import torch
+    page, lens, window = 16, [37, 90, 16], 21
+    cache = _cache(rb, 16, 2, page, 64, 4)
+    table = torch.full((3, 6), 1 << 30, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(16).tolist()
+    seen = torch.zeros(16, page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            table[b, i] = ids.pop()
+        for k in range(max(0, n - window), n):
+            seen[table[b, k // page].item(), k % page] = True
+    kc, ks, vc, vs, _, _ = cache.tensors
+    clean = _check(rb, cache, t, lens, [1, 1, 1], 4, window=window, table=table)
+    for s in (ks, vs):
+        s.transpose(1, 2)[~seen.cuda()] = 0x7F
+    q, O, *_ = _attend(rb, cache, t, lens, [1, 1, 1], 4, window=window, table=table)
+    rb.sync_status()
+    assert torch.equal(O, clean)
+    table[1, 0] = -1  # a page wholly before the window may be gone
+    _, O, *_ = _attend(rb, cache, t, lens, [1, 1, 1], 4, window=window, table=table)
+    rb.sync_status()
+    assert torch.equal(O, clean)
+
+
+def test_bad_pages_are_reported_and_taken_as_masked(rb, cuda):
+    import torch
+    cache = _cache(rb, 8, 1, 16, 64, 2)
+    table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(2, 4)
+    lens = torch.tensor([64, 50], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda")
+    good = rb.attention_kv4(q, cache, lens, table)
+    rb.sync_status()
+    for bad in (-1, 8, 2147483647, -2147483648):
+        broken = table.clone()
+        broken[0, 1] = bad
+        O = rb.attention_kv4(q, cache, lens, broken)
+        with pytest.raises(rb.RougeB200Error) as e:
+            rb.sync_status()
+        assert e.value.status == rb.EINVAL
+        assert torch.equal(O[1], good[1]) and O.isfinite().all()
+    # a length past the table: the keys that have a page count
+    O = rb.attention_kv4(q, cache, torch.tensor([1000, 50], dtype=torch.int32, device="cuda"), table)
+    with pytest.raises(rb.RougeB200Error):
+        rb.sync_status()
+    assert torch.equal(O[1], good[1]) and (O[0] - good[0]).abs().max() < 1e-5
+    rb.sync_status()
+
+
+def test_same_call_same_bits_and_shared_pages(rb, cuda):
+    import torch
+    cache = _cache(rb, 70, 2, 64, 128, 6)
+    table = torch.arange(70, dtype=torch.int32, device="cuda").repeat(3, 1)  # (three sequences on the same pages)
+    lens = [4400, 4480, 1000]
+    q, O, _, lens_d, _ = _attend(rb, cache, "bf16", lens, [1, 1, 1], 16, table=table)
+    for _ in range(5):
+        assert torch.equal(rb.attention_kv4(q, cache, lens_d, table), O)
+    rb.sync_status()
+
+
+def test_captured_replayed_and_on_another_stream(rb, cuda):
+    """One capture serves growing lengths; two streams at a time need two workspaces."""
+    import torch
+    cache = _cache(rb, 64, 2, 32, 64, 5)
+    table = torch.arange(64, dtype=torch.int32, device="cuda").reshape(2, 32)
+    q = torch.randn(2, 8, 64, device="cuda").bfloat16()
+    lens = torch.tensor([3, 40], dtype=torch.int32, device="cuda")
+    n = rb.attention_kv4_workspace(2, 8, 2, 64, 1, 1024, rb.T_BF16)
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    out = torch.empty_like(q)
+    rb.attention_kv4(q, cache, lens, table, O=out, workspace=ws[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rb.attention_kv4(q, cache, lens, table, O=out, workspace=ws[0])
+    side = torch.cuda.Stream()
+    for a, b in ((3, 40), (1000, 1024), (0, 1)):
+        lens.copy_(torch.tensor([a, b]))
+        want = rb.attention_kv4(q, cache, lens, table)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = rb.attention_kv4(q, cache, lens, table, workspace=ws[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(other, want)
+    rb.sync_status()
+
+
+def test_workspace_is_checked(rb, cuda):
+    import torch
+    cache = _cache(rb, 4, 1, 16, 64, 5)
+    q, lens = torch.randn(1, 2, 64, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    n = rb.attention_kv4_workspace(1, 2, 1, 64, 1, 64, rb.T_F32)
+    with pytest.raises(rb.RougeB200Error) as e:
+        rb.attention_kv4(q, cache, lens, table, workspace=torch.empty(n - 1, dtype=torch.uint8, device="cuda"))
+    assert e.value.status == rb.ETOOBIG
+
+
+def test_decoder_step_together(rb, cuda):
+    """norm -> int8 QKV product with bias -> cache write -> attention over the cache -> output product with the
+    residual, three tokens in a row, against the same steps in f32 / 64 bits from the intermediate codes."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(0)
+    B, D, Hq, Hkv, Dh, page = 5, 256, 8, 2, 64, 16
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    N = (Hq + 2 * Hkv) * Dh
+    wqkv, wo, bias, wn = rn(N, D) / 16, rn(D, Hq * Dh) / 23, rn(N), 0.5 + torch.rand(D, generator=g, device="cuda")
+
+    def q8(w):
+        q, s = torch.empty(w.shape, dtype=torch.int8, device="cuda"), torch.empty(w.shape[0], device="cuda")
+        rb.quantize_i8_rows(w.contiguous(), s, q)
+        return q, s
+    qkv_q, qkv_s = q8(wqkv)
+    o_q, o_s = q8(wo)
+    cache = rb.KV4Cache.empty(8, Hkv, page, Dh)
+    table = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    res = rn(B, D).bfloat16()
+    for step in range(3):
+        x = rn(B, D).bfloat16()
+        h, codes, scales = torch.empty_like(x), torch.empty(B, D, dtype=torch.int8, device="cuda"), torch.empty(
+            B, device="cuda")
+        rb.add_rmsnorm_quant(x, res, wn, 1e-5, rb.Q_I8_ROWS, codes, scales, h)
+        qkv = torch.empty(B, N, dtype=torch.bfloat16, device="cuda")
+        rb.gemm_i8(codes, qkv_q, rb.B_NK, qkv, rb.OUT_BF16, scales, 1, qkv_s, 1, epilogue=rb.Epilogue(bias))
+        q = qkv[:, :Hq * Dh].reshape(B, Hq, Dh).contiguous()
+        k, v = qkv[:, Hq * Dh:(Hq + Hkv) * Dh].unflatten(1, (Hkv, Dh)), qkv[:, (Hq + Hkv) * Dh:].unflatten(1, (Hkv, Dh))
+        rb.kv4_write(cache, k, v, table[:, 0] * page + lens)
+        lens += 1
+        att = rb.attention_kv4(q, cache, lens, table)
+        aq, asc = q8(att.reshape(B, Hq * Dh).float())
+        out = h.clone()
+        rb.gemm_i8(aq, o_q, rb.B_NK, out, rb.OUT_BF16, asc, 1, o_s, 1, epilogue=rb.Epilogue(residual=out))
+        rb.sync_status()
+        # each step from the one before it
+        want_h = (x.float() + res.float()).bfloat16()
+        assert torch.equal(h, want_h)
+        wq = (codes.double() @ qkv_q.double().T) * scales.double()[:, None] * qkv_s.double() + bias.double()
+        assert ((qkv.double() - wq).abs() <= wq.abs() * 2.0 ** -8 + 2.0 ** -20).all()
+        ref, spread, ds, _ = _reference(cache, q, [step + 1] * B, table, [1] * B, 1, 0, 1 / 8)
+        assert ((att.double() - ref).abs() <= (2 * ds + 2.0 ** -10) * spread + ref.abs() * 2.0 ** -8).all()
+        wo_ = (aq.double() @ o_q.double().T) * asc.double()[:, None] * o_s.double() + h.double()
+        assert ((out.double() - wo_).abs() <= wo_.abs() * 2.0 ** -8 + 2.0 ** -20).all()
+        res = out
