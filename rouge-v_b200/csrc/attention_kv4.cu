@@ -40,7 +40,6 @@ namespace rb200 {
 namespace {
 
 constexpr int kTile = 32;   // keys per tile
-constexpr int kWarps = 8;   // per CTA
 constexpr int kMinTiles = 2;  // tiles per warp before another warp joins
 
 struct AttnArgs {
@@ -58,7 +57,7 @@ struct AttnArgs {
   float scale;
   int causal, window;
   int warps;      // warps of the grid
-  float *part;    // [2 * warps][rows][Dh + 2]: weighted sums, then maximum and sum per row
+  float *part;    // [2 * warps][rows * (Dh + 4)]: weighted sums, then maximum and sum per row
   int4 *desc;     // [2 * warps]: sequence, head, row tile, valid
   int *err;
 };
@@ -90,8 +89,7 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) 
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -109,28 +107,40 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
+// Key (of 16) in row r of the score products' A fragments. Lane t's rows 2t,
+// 2t + 1, 2t + 8 and 2t + 9 of the weights hold the keys t, 4 + (t ^ 1), and
+// 8 more: the four value rows a load reads then lie in two bank halves, and
+// so do the two key rows that eight lanes read together.
+__device__ __forceinline__ int key_of_row(int r) {
+  const int q = (r & 7) >> 1;
+  return (r & 8) + ((r & 1) ? 4 + (q ^ 1) : q);
 }
 
+// 16 consecutive query values (16-byte aligned).
 template <int T>
-__device__ __forceinline__ float load_q(const void *q, long long at) {
-  if constexpr (T == ROUGE_B200_T_F32) return static_cast<const float *>(q)[at];
-  const uint16_t h = static_cast<const uint16_t *>(q)[at];
-  if constexpr (T == ROUGE_B200_T_F16) return __half2float(__ushort_as_half(h));
-  return __uint_as_float(static_cast<uint32_t>(h) << 16);
+__device__ __forceinline__ void load_q16(const void *q, long long at, float *v) {
+  if constexpr (T == ROUGE_B200_T_F32) {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 t = p[i];
+      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+    }
+  } else {
+    const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + at);
+    const uint4 t0 = p[0], t1 = p[1];
+    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (T == ROUGE_B200_T_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      }
+    }
+  }
 }
 
 template <int T>
@@ -143,6 +153,11 @@ __device__ __forceinline__ void store_o(void *o, long long at, float v) {
     static_cast<uint16_t *>(o)[at] = static_cast<uint16_t>(bf16x2_rn(v, 0.0f));
 }
 
+// Warps per block and blocks per SM: 16 warps an SM where a warp's O^T
+// accumulators and queries leave it 128 registers, 12 with 168, 8 with 255.
+constexpr int warps_of(int Dh, int nt) { return Dh > 128 || nt == 1 ? 8 : 12; }
+constexpr int ctas_of(int Dh, int nt) { return Dh > 128 || nt == 2 ? 1 : 2; }
+
 // DT: Dh rounded up to 64, 128 or 256. NT: tiles of 8 mma columns. f32
 // queries: columns 8.. hold the low parts of rows 0.., so 4 * NT rows.
 template <int DT, int NT, int T>
@@ -151,16 +166,20 @@ struct Shape {
   static constexpr int NR = SPLIT ? NT / 2 : NT;  // column tiles of distinct rows
   static constexpr int ROWS = 8 * NR;
   static constexpr int STAGES = DT == 256 ? 2 : 3;
+  static constexpr int WARPS = warps_of(DT, NT);
+  static constexpr int CTAS = ctas_of(DT, NT);
   static_assert(!SPLIT || NT % 2 == 0, "two parts");
 };
 
 // Bytes of one stage: codes and scales of K and V of one tile.
 __host__ __device__ __forceinline__ int stage_bytes(int Dh) { return kTile * Dh * 9 / 8; }
 
-template <int DT, int NT, int T>
-__global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
+// FULL: Dh == DT, every size a constant.
+template <int DT, int NT, int T, bool FULL>
+__global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     attention_kv4_kernel(const AttnArgs a) {
   using S = Shape<DT, NT, T>;
+  constexpr int kWarps = S::WARPS;
   constexpr int kBlk = DT / 64;      // K scale blocks per lane (a run of DT / 4 values)
   constexpr int kSteps = DT / 16;    // mma steps over d
   constexpr int kMt = DT / 16;       // O^T row tiles
@@ -218,12 +237,14 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
 
-  const int cb = a.Dh / 2, sbk = a.Dh / 16;  // bytes per key: codes, scales
-  const int nblk = a.Dh / 16;
-  const int stage_sz = stage_bytes(a.Dh);
+  const int Dh = FULL ? DT : a.Dh;
+  const int cb = Dh / 2, sbk = Dh / 16;  // bytes per key: codes, scales
+  const int nblk = Dh / 16;
+  const int stage_sz = stage_bytes(Dh);
   uint8_t *ring = smem + static_cast<size_t>(warp) * S::STAGES * stage_sz;
-  const uint32_t ring_u = smem_u32(ring);
   const volatile int never = 0;
+  const int k_row = key_of_row(g);                                  // + 8: the lane's other row
+  const int v_row[2] = {key_of_row(2 * t), key_of_row(2 * t + 1)};  // + 8: two more
   uint32_t it = 0;  // tiles taken from the ring so far
   bool alive = true;
 
@@ -324,15 +345,21 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
         const int r = r0 + j * 8 + g;
         const bool live = r < nrows;
         const int qi = si.q0 + (live ? r / a.group : 0), h = hk * a.group + (live ? r % a.group : 0);
-        const long long at = (static_cast<long long>(qi) * a.Hq + h) * a.Dh;
+        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh;
         float v[DT / 4];
         float m = 0.0f;
 #pragma unroll
-        for (int k = 0; k < DT / 4; ++k) {
-          const int d = t * (DT / 4) + k;
-          v[k] = live && d < a.Dh ? load_q<T>(a.Q, at + d) : 0.0f;
-          m = fmaxf(m, fabsf(v[k]));
+        for (int k = 0; k < kBlk; ++k) {
+          const int d = t * (DT / 4) + 16 * k;
+          if (live && (FULL || d < Dh)) {
+            load_q16<T>(a.Q, at + d, v + 16 * k);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[16 * k + i] = 0.0f;
+          }
         }
+#pragma unroll
+        for (int k = 0; k < DT / 4; ++k) m = fmaxf(m, fabsf(v[k]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
         // exponent of the row maximum (0 for an empty or unbounded row)
@@ -351,7 +378,8 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
               qf[S::NR + j][s][p] = f16x2_rn(x0 - b2.x, x1 - b2.y);
             }
           }
-        const float mine = scalbnf(a.scale * 1.44269504f * gk, e);
+        // (kept positive: a masked score is -inf before it is scaled)
+        const float mine = fmaxf(scalbnf(a.scale * 1.44269504f * gk, e), 1e-37f);
         mult[j][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
         mult[j][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
       }
@@ -385,8 +413,8 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
         alive = false;
         break;
       }
-      const uint32_t kc = ring_u + s * stage_sz, vc = kc + kTile * cb;
-      const uint32_t ks = kc + 2 * kTile * cb, vs = ks + kTile * sbk;
+      const uint8_t *kc = ring + s * stage_sz, *vc = kc + kTile * cb;
+      const uint8_t *ks = kc + 2 * kTile * cb, *vs = ks + kTile * sbk;
       const int key0 = tile * kTile;
       const bool masked = ok != 3u || key0 + kTile > hi_min || key0 < lo_max;
 
@@ -398,43 +426,76 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[kb][j][e] = 0.0f;
-        const uint32_t row0 = kb * 16 + g;
+        uint32_t w[2][2 * kBlk], sx[2][kBlk];  // codes and scales (f16 pairs) of rows g, g + 8
 #pragma unroll
-        for (int blk = 0; blk < kBlk; ++blk) {
-          const int gb = t * kBlk + blk;  // block of 16 values
-          uint2 w0 = make_uint2(0u, 0u), w1 = w0;
-          uint32_t s0 = 0, s1 = 0;
-          if (gb < nblk) {
-            w0 = lds64(kc + row0 * cb + gb * 8);
-            w1 = lds64(kc + (row0 + 8) * cb + gb * 8);
-            s0 = lds8(ks + row0 * sbk + gb);
-            s1 = lds8(ks + (row0 + 8) * sbk + gb);
-          }
-          const uint32_t sh = e4m3x2_f16x2(s0 | (s1 << 8));
-          const uint32_t sa = __byte_perm(sh, sh, 0x1010), sb = __byte_perm(sh, sh, 0x3232);
+        for (int u = 0; u < 2; ++u) {
+          const int row = kb * 16 + u * 8 + k_row;
+          const uint8_t *pc = kc + row * cb + t * (DT / 8), *ps = ks + row * sbk + t * kBlk;
+          if constexpr (FULL && kBlk >= 2) {
 #pragma unroll
-          for (int hw = 0; hw < 2; ++hw) {
-            uint32_t x[4], y[4];
-            e2m1x8_f16x2(hw ? w0.y : w0.x, x);
-            e2m1x8_f16x2(hw ? w1.y : w1.x, y);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              x[q] = mul_f16x2(x[q], sa);
-              y[q] = mul_f16x2(y[q], sb);
+            for (int q = 0; q < kBlk / 2; ++q) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(pc + 16 * q);
+              w[u][4 * q] = v.x; w[u][4 * q + 1] = v.y; w[u][4 * q + 2] = v.z; w[u][4 * q + 3] = v.w;
+              const uint32_t h = e4m3x2_f16x2(*reinterpret_cast<const uint16_t *>(ps + 2 * q));
+              sx[u][2 * q] = __byte_perm(h, h, 0x1010);
+              sx[u][2 * q + 1] = __byte_perm(h, h, 0x3232);
             }
+          } else {
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              const int step = blk * 4 + hw * 2 + k2;
-#pragma unroll
-              for (int j = 0; j < NT; ++j)
-                mma16816(sc[kb][j], x[2 * k2], y[2 * k2], x[2 * k2 + 1], y[2 * k2 + 1],
-                         qf[j][step][0], qf[j][step][1]);
+            for (int q = 0; q < kBlk; ++q) {
+              uint2 v = make_uint2(0u, 0u);
+              uint32_t h = 0;
+              if (FULL || t * kBlk + q < nblk) {
+                v = *reinterpret_cast<const uint2 *>(pc + 8 * q);
+                h = e4m3x2_f16x2(ps[q]);
+              }
+              w[u][2 * q] = v.x; w[u][2 * q + 1] = v.y;
+              sx[u][q] = __byte_perm(h, h, 0x1010);
             }
           }
         }
+#pragma unroll
+        for (int q = 0; q < 2 * kBlk; ++q) {
+          uint32_t x[4], y[4];
+          e2m1x8_f16x2(w[0][q], x);
+          e2m1x8_f16x2(w[1][q], y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = mul_f16x2(x[i], sx[0][q / 2]);
+            y[i] = mul_f16x2(y[i], sx[1][q / 2]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              mma16816(sc[kb][j], x[2 * i], y[2 * i], x[2 * i + 1], y[2 * i + 1],
+                       qf[j][2 * q + i][0], qf[j][2 * q + i][1]);
+        }
       }
 
-      // ---- softmax step: lane columns 2t, 2t + 1, keys g and g + 8 of each 16
+      // ---- softmax step: lane columns 2t, 2t + 1, key rows g and g + 8 of each 16
+      if constexpr (S::SPLIT) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < S::NR; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[kb][j][e] += sc[kb][S::NR + j][e];
+      }
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int key = key0 + kb * 16 + u * 8 + k_row;
+#pragma unroll
+            for (int j = 0; j < S::NR; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (!((ok >> kb) & 1u) || key >= col_hi[j][e] || key < col_lo[j][e])
+                  sc[kb][j][2 * u + e] = -INFINITY;
+          }
+      }
       uint32_t pf[2][NT][2];
       bool grow = false;
       float nm[S::NR][2];
@@ -442,26 +503,12 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
       for (int j = 0; j < S::NR; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float m = mx[j][e];
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float v = sc[kb][j][2 * u + e];
-              if constexpr (S::SPLIT) v += sc[kb][S::NR + j][2 * u + e];
-              v *= mult[j][e];
-              if (masked) {
-                const int key = key0 + kb * 16 + u * 8 + g;
-                if (!((ok >> kb) & 1u) || key >= col_hi[j][e] || key < col_lo[j][e]) v = -INFINITY;
-              }
-              sc[kb][j][2 * u + e] = v;
-              m = fmaxf(m, v);
-            }
+          float m = fmaxf(fmaxf(sc[0][j][e], sc[0][j][2 + e]), fmaxf(sc[1][j][e], sc[1][j][2 + e]));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          nm[j][e] = m;
-          grow |= m > mx[j][e];
+          nm[j][e] = m * mult[j][e];
+          grow |= nm[j][e] > mx[j][e];
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -469,7 +516,7 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float f = nm[j][e] > mx[j][e] ? ex2(mx[j][e] - nm[j][e]) : 1.0f;
-            mx[j][e] = nm[j][e];
+            mx[j][e] = fmaxf(mx[j][e], nm[j][e]);
             sum[j][e] *= f;
 #pragma unroll
             for (int m = 0; m < kMt; ++m) {
@@ -489,12 +536,12 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
         for (int e = 0; e < 2; ++e) {
           // (weights carry a factor 2^15, which the division by their sum
           // takes out: f16 then keeps 11 bits of weights down to 2^-29)
-          const float m = mx[j][e] == -INFINITY ? 0.0f : mx[j][e] - 15.0f;
+          const float m = mx[j][e] == -INFINITY ? 0.0f : 15.0f - mx[j][e];
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              p[kb][2 * u + e] = ex2(sc[kb][j][2 * u + e] - m);
+              p[kb][2 * u + e] = ex2(__fmaf_rn(sc[kb][j][2 * u + e], mult[j][e], m));
               sum[j][e] += p[kb][2 * u + e];
             }
         }
@@ -512,37 +559,50 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
           }
       }
 
-      // ---- weighted sums: lane keys 2t, 2t + 1, 2t + 8, 2t + 9, values d = g * DT / 8 + ...
+      // ---- weighted sums: the lane's keys of weight rows 2t, 2t + 1, 2t + 8,
+      // 2t + 9, values d = g * DT / 8 + ...
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const uint32_t rows[4] = {kb * 16 + 2u * t, kb * 16 + 2u * t + 1, kb * 16 + 2u * t + 8,
-                                  kb * 16 + 2u * t + 9};
+        constexpr int kSb = DT == 256 ? 2 : 1;  // scale blocks of the lane's values
+        uint32_t c[4][kVw], sv[4][kSb];
 #pragma unroll
-        for (int w = 0; w < kVw; ++w) {
-          const int e0 = g * (DT / 8) + 8 * w;  // first value of this word
-          uint32_t c[4] = {0, 0, 0, 0}, sv[4] = {0, 0, 0, 0};
-          if (e0 < a.Dh) {
+        for (int q = 0; q < 4; ++q) {
+          const int row = kb * 16 + v_row[q & 1] + (q & 2) * 4;
+          const uint8_t *pc = vc + row * cb + g * (DT / 16);
+          const uint8_t *ps = vs + row * sbk + (DT == 64 ? g / 2 : g * kSb);
+          if constexpr (FULL && kVw == 2) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(pc);
+            c[q][0] = v.x; c[q][1] = v.y;
+          } else if constexpr (FULL && kVw == 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(pc);
+            c[q][0] = v.x; c[q][1] = v.y; c[q][2] = v.z; c[q][3] = v.w;
+          } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              c[q] = lds32(vc + rows[q] * cb + e0 / 2);
-              sv[q] = lds8(vs + rows[q] * sbk + e0 / 16);
-            }
-            if (masked) {  // keys of no row: a zero scale, whatever the page holds
+            for (int w = 0; w < kVw; ++w)
+              c[q][w] = FULL || g * (DT / 8) + 8 * w < Dh
+                            ? *reinterpret_cast<const uint32_t *>(pc + 4 * w) : 0u;
+          }
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int key = key0 + static_cast<int>(rows[q]);
-                if (!((ok >> kb) & 1u) || key >= hi_max || key < lo_min) sv[q] = 0;
-              }
+          for (int w = 0; w < kSb; ++w)
+            sv[q][w] = FULL || g * (DT / 8) + 16 * w < Dh ? ps[w] : 0u;
+          if (masked) {  // keys of no row: a zero scale, whatever the page holds
+            const int key = key0 + row;
+            if (!((ok >> kb) & 1u) || key >= hi_max || key < lo_min) {
+#pragma unroll
+              for (int w = 0; w < kSb; ++w) sv[q][w] = 0u;
             }
           }
-          const uint32_t s01 = e4m3x2_f16x2(sv[0] | (sv[1] << 8));
-          const uint32_t s23 = e4m3x2_f16x2(sv[2] | (sv[3] << 8));
+        }
+#pragma unroll
+        for (int w = 0; w < kVw; ++w) {
+          const uint32_t s01 = e4m3x2_f16x2(sv[0][w * kSb / kVw] | (sv[1][w * kSb / kVw] << 8));
+          const uint32_t s23 = e4m3x2_f16x2(sv[2][w * kSb / kVw] | (sv[3][w * kSb / kVw] << 8));
           constexpr uint32_t kLo = 0x0F0F0F0Fu;
           uint32_t ev01[4], od01[4], ev23[4], od23[4];
-          e2m1x8_f16x2((c[0] & kLo) | ((c[1] << 4) & ~kLo), ev01);
-          e2m1x8_f16x2(((c[0] >> 4) & kLo) | (c[1] & ~kLo), od01);
-          e2m1x8_f16x2((c[2] & kLo) | ((c[3] << 4) & ~kLo), ev23);
-          e2m1x8_f16x2(((c[2] >> 4) & kLo) | (c[3] & ~kLo), od23);
+          e2m1x8_f16x2((c[0][w] & kLo) | ((c[1][w] << 4) & ~kLo), ev01);
+          e2m1x8_f16x2(((c[0][w] >> 4) & kLo) | (c[1][w] & ~kLo), od01);
+          e2m1x8_f16x2((c[2][w] & kLo) | ((c[3][w] << 4) & ~kLo), ev23);
+          e2m1x8_f16x2(((c[2][w] >> 4) & kLo) | (c[3][w] & ~kLo), od23);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const uint32_t a0 = mul_f16x2(ev01[q], s01), a1 = mul_f16x2(od01[q], s01);
@@ -564,7 +624,7 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
     // ---- sums over the lanes of a column, then the unit's result or its part
     const float gv = a.gs_v ? __ldg(a.gs_v + hk) : 1.0f;
     const int slot = 2 * gw + (first == 0 ? 1 : 0);
-    float *part = a.part + static_cast<size_t>(slot) * S::ROWS * (a.Dh + 2);
+    float *part = a.part + static_cast<size_t>(slot) * S::ROWS * (Dh + 4);
     if (!whole && lane == 0) a.desc[slot] = make_int4(b, hk, rt, 1);
 #pragma unroll
     for (int j = 0; j < S::NR; ++j)
@@ -578,50 +638,53 @@ __global__ void __launch_bounds__(kWarps * 32, DT == 256 || NT > 2 ? 1 : 2)
         if (r >= nrows) continue;
         const float f = whole ? (l > 0.0f || l != l ? gv / l : 0.0f) : 1.0f;
         const int qi = si.q0 + r / a.group, h = hk * a.group + r % a.group;
-        const long long at = (static_cast<long long>(qi) * a.Hq + h) * a.Dh;
+        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh;
 #pragma unroll
         for (int m = 0; m < kMt; ++m)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int d = g * (DT / 8) + 2 * m + u;
-            if (d >= a.Dh) continue;
+            if (!FULL && d >= Dh) continue;
             float v = o[j][m][2 * u + e];
             if constexpr (S::SPLIT) v += o[S::NR + j][m][2 * u + e];
             if (whole)
               store_o<T>(a.O, at + d, v * f);
             else
-              part[rr * a.Dh + d] = v;
+              part[rr * Dh + d] = v;
           }
         if (!whole && g == 0) {
-          part[S::ROWS * a.Dh + rr] = mx[j][e];
-          part[S::ROWS * (a.Dh + 1) + rr] = l;
+          part[S::ROWS * Dh + rr] = mx[j][e];
+          part[S::ROWS * (Dh + 1) + rr] = l;
         }
       }
   }
 }
 
-// Joins the parts of a unit that several warps computed: block (w, row)
-// handles the unit whose first part is slot 2w + 1; the others are the
-// first slots of the warps after it. Order and so rounding are fixed.
+// Joins the parts of the units that several warps computed: block (w, y)
+// handles the unit whose first part is slot 2w + 1 -- the others are the
+// first slots of the warps after it -- and, of its rows, the y-th of
+// gridDim.y shares. Order and so rounding are fixed.
 constexpr int kJoinThreads = 256;
 
 template <int T>
 __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const AttnArgs a, int rows) {
-  __shared__ float red[kJoinThreads];
-  __shared__ float acc[kJoinThreads];
+  __shared__ float4 acc[kJoinThreads];
+  __shared__ float weight_sum[kJoinThreads];
+  __shared__ float row_max[16];
   grid_dependency_wait();
-  const int w0 = blockIdx.x, rr = blockIdx.y;
+  const int w0 = blockIdx.x, tid = threadIdx.x;
   const int4 u = a.desc[2 * w0 + 1];
   if (!u.w) return;
   const int q0 = a.cu_q ? a.cu_q[u.x] : u.x;
   int nq = a.cu_q ? a.cu_q[u.x + 1] - q0 : 1;
   nq = max(0, min(nq, a.max_q));
-  const int r = u.z * rows + rr;
-  if (r >= nq * a.group) return;
+  const int share = rows / gridDim.y, first = blockIdx.y * share;
+  const int live = min(share, nq * a.group - u.z * rows - first);  // this block's rows
+  if (live <= 0) return;
   // parts of the unit: the first slots of w0 + 1 .. that carry it
   int n = 1;
   for (;;) {
-    const int i = w0 + n + static_cast<int>(threadIdx.x);
+    const int i = w0 + n + tid;
     bool same = false;
     if (i < a.warps) {
       const int4 d = a.desc[2 * i];
@@ -631,51 +694,57 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
     n += c;
     if (c < kJoinThreads) break;
   }
-  const size_t stride = static_cast<size_t>(rows) * (a.Dh + 2);
+  const size_t stride = static_cast<size_t>(rows) * (a.Dh + 4);
   auto part = [&](int i) { return a.part + (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * stride; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) m = fmaxf(m, part(i)[rows * a.Dh + rr]);
-  red[threadIdx.x] = m;
-  __syncthreads();
-  for (int o = kJoinThreads / 2; o; o >>= 1) {
-    if (threadIdx.x < o) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + o]);
-    __syncthreads();
-  }
-  m = red[0] == -INFINITY ? 0.0f : red[0];
-  // kJoinThreads / lanes groups of parts, each lane of a group 4 values of d
-  const int lanes = (a.Dh + 3) / 4, groups = kJoinThreads / lanes;
-  const int grp = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
-  const float gv = a.gs_v ? a.gs_v[u.y] : 1.0f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.0f;
-  if (grp < groups) {
-    for (int i = grp; i < n; i += groups) {
-      const float *p = part(i);
-      const float f = ex2(p[rows * a.Dh + rr] - m);
-      const float2 x = *reinterpret_cast<const float2 *>(p + rr * a.Dh + d);
-      const float2 y = *reinterpret_cast<const float2 *>(p + rr * a.Dh + d + 2);
-      l += f * p[rows * (a.Dh + 1) + rr];
-      v.x += f * x.x; v.y += f * x.y; v.z += f * y.x; v.w += f * y.y;
-    }
-  }
-  const int h = u.y * a.group + r % a.group;
-  const long long at = (static_cast<long long>(q0 + r / a.group) * a.Hq + h) * a.Dh;
-  const float *vals[4] = {&v.x, &v.y, &v.z, &v.w};
-  __syncthreads();
-  red[threadIdx.x] = l;
+  for (int r = tid >> 5; r < live; r += kJoinThreads / 32) {
+    float m = -INFINITY;
+    for (int i = tid & 31; i < n; i += 32) m = fmaxf(m, part(i)[rows * a.Dh + first + r]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    acc[threadIdx.x] = *vals[k];
-    __syncthreads();
-    if (threadIdx.x < lanes) {
-      float s = 0.0f, tl = 0.0f;
-      for (int q = 0; q < groups; ++q) {
-        s += acc[q * lanes + threadIdx.x];
-        tl += red[q * lanes + threadIdx.x];
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((tid & 31) == 0) row_max[r] = m == -INFINITY ? 0.0f : m;
+  }
+  __syncthreads();
+  // a thread holds 4 values of d of one row, over every groups-th part
+  const int lanes = a.Dh / 4, per_row = kJoinThreads / lanes;
+  const int rows_at_once = live < per_row ? live : per_row, groups = per_row / rows_at_once;
+  const int d = (tid % lanes) * 4, slot = tid / lanes;
+  const float gv = a.gs_v ? a.gs_v[u.y] : 1.0f;
+  for (int r0 = 0; r0 < live; r0 += rows_at_once) {
+    const int r = r0 + slot % rows_at_once, grp = slot / rows_at_once;
+    const bool on = grp < groups && r < live && slot < per_row;
+    const int rr = first + r;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+    if (on) {
+      const float m = row_max[r];
+#pragma unroll 4
+      for (int i = grp; i < n; i += groups) {
+        const float *p = part(i);
+        const float f = ex2(p[rows * a.Dh + rr] - m);
+        const float4 x = *reinterpret_cast<const float4 *>(p + rr * a.Dh + d);
+        l += f * p[rows * (a.Dh + 1) + rr];
+        v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
       }
-      if (d + k < a.Dh) store_o<T>(a.O, at + d + k, (tl > 0.0f || tl != tl) ? s * (gv / tl) : 0.0f);
     }
     __syncthreads();
+    acc[tid] = v;
+    weight_sum[tid] = l;
+    __syncthreads();
+    if (on && grp == 0) {
+      for (int q = 1; q < groups; ++q) {
+        const int o = tid + q * rows_at_once * lanes;
+        v.x += acc[o].x; v.y += acc[o].y; v.z += acc[o].z; v.w += acc[o].w;
+        l += weight_sum[o];
+      }
+      const float f = (l > 0.0f || l != l) ? gv / l : 0.0f;
+      const int row = u.z * rows + rr;
+      const long long at =
+          (static_cast<long long>(q0 + row / a.group) * a.Hq + u.y * a.group + row % a.group) * a.Dh + d;
+      store_o<T>(a.O, at, v.x * f);
+      store_o<T>(a.O, at + 1, v.y * f);
+      store_o<T>(a.O, at + 2, v.z * f);
+      store_o<T>(a.O, at + 3, v.w * f);
+    }
   }
 }
 
@@ -685,53 +754,62 @@ int rows_of(int group, int max_q, int type) {
   return rows <= 8 ? 8 : 16;
 }
 
-// Warps of the grid: two CTAs per SM (one for heads above 128), fewer where
-// even the longest sequences would leave warps without kMinTiles tiles.
+// mma column tiles per warp (see Shape).
+int nt_of(int rows, int type) { return type == ROUGE_B200_T_F32 || rows == 16 ? 2 : 1; }
+
+// Warps of the grid: every SM's, fewer where even the longest sequences
+// would leave warps without kMinTiles tiles.
 int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, int type) {
-  const long long rts = (static_cast<long long>(group) * max_q + rows_of(group, max_q, type) - 1) /
-                        rows_of(group, max_q, type);
-  const long long tiles = max_kv < kTile ? 1 : (max_kv + kTile - 1) / kTile;
-  const long long cap = static_cast<long long>(current_sm_count()) * (Dh > 128 ? 1 : 2);
-  // (products kept below 2^63: each factor is below 2^31)
-  long long want = cap;
-  const long long units = static_cast<long long>(B) * Hkv;
-  if (units < cap * kWarps * kMinTiles && rts < cap * kWarps * kMinTiles) {
-    const double all = static_cast<double>(units) * rts * tiles / kMinTiles / kWarps;
-    if (all < static_cast<double>(cap)) want = static_cast<long long>(std::ceil(all));
-  }
-  return static_cast<int>(want < 1 ? 1 : want) * kWarps;
+  const int rows = rows_of(group, max_q, type), nt = nt_of(rows, type), warps = warps_of(Dh, nt);
+  const double rts = std::ceil(static_cast<double>(group) * max_q / rows);
+  const double tiles = max_kv < kTile ? 1.0 : std::ceil(static_cast<double>(max_kv) / kTile);
+  const int cap = current_sm_count() * ctas_of(Dh, nt);
+  const double want = std::ceil(static_cast<double>(B) * Hkv * rts * tiles / kMinTiles / warps);
+  return (want < cap ? static_cast<int>(want) : cap) * warps;
 }
 
 size_t part_bytes(int warps, int rows, int Dh) {
-  return round_up(static_cast<size_t>(2) * warps * rows * (Dh + 2) * 4, 256);
+  return round_up(static_cast<size_t>(2) * warps * rows * (Dh + 4) * 4, 256);
 }
 
-template <int DT, int NT, int T>
-int launch_shape(const AttnArgs &a, cudaStream_t st) {
+template <int DT, int NT, int T, bool FULL>
+int launch_kernels(const AttnArgs &a, int join_y, cudaStream_t st) {
   using S = Shape<DT, NT, T>;
-  auto kern = attention_kv4_kernel<DT, NT, T>;
-  const int smem = kWarps * S::STAGES * stage_bytes(a.Dh);
+  auto kern = attention_kv4_kernel<DT, NT, T, FULL>;
+  const int smem = S::WARPS * S::STAGES * stage_bytes(a.Dh);
   static std::atomic<unsigned long long> attr_done{0};
   const unsigned long long bit = 1ull << (current_device() & 63);
   if (!(attr_done.load() & bit)) {
     const int s = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kWarps * S::STAGES * stage_bytes(DT)));
+                                                   S::WARPS * S::STAGES * stage_bytes(DT)));
     if (s != ROUGE_B200_OK) return s;
     attr_done.fetch_or(bit);
   }
-  kern<<<a.warps / kWarps, kWarps * 32, smem, st>>>(a);
+  kern<<<a.warps / S::WARPS, S::WARPS * 32, smem, st>>>(a);
   int s = cuda_status(cudaGetLastError());
   if (s != ROUGE_B200_OK) return s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.warps, S::ROWS, 1);
+  cfg.gridDim = dim3(a.warps, join_y, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, attention_kv4_join_kernel<T>, a, static_cast<int>(S::ROWS)));
+}
+
+template <int DT, int NT, int T>
+int launch_shape(const AttnArgs &a, cudaStream_t st) {
+  // A block joins all rows of a unit, or, where a unit may be cut into more
+  // than 16 parts (few units), one row.
+  const double units = static_cast<double>(a.B) * a.Hkv *
+                       ((static_cast<double>(a.max_q) * a.group + Shape<DT, NT, T>::ROWS - 1) /
+                        Shape<DT, NT, T>::ROWS);
+  const int join_y = a.warps > 16 * units ? Shape<DT, NT, T>::ROWS : 1;
+  return a.Dh == DT ? launch_kernels<DT, NT, T, true>(a, join_y, st)
+                    : launch_kernels<DT, NT, T, false>(a, join_y, st);
 }
 
 template <int DT>
