@@ -40,7 +40,7 @@ namespace rb200 {
 namespace {
 
 constexpr int kTile = 32;   // keys per tile
-constexpr int kMinTiles = 2;  // tiles per warp before another warp joins
+constexpr int kMinTilesLog2 = 1;  // two tiles per warp before another warp joins
 
 struct AttnArgs {
   const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
@@ -86,6 +86,15 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) 
   s.work = static_cast<long long>(s.tiles) * s.rts * a.Hkv;
   return s;
 }
+
+// a / b for a >= 0, b > 0: the 32-bit division where it fits.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -143,14 +152,17 @@ __device__ __forceinline__ void load_q16(const void *q, long long at, float *v) 
   }
 }
 
+// Four consecutive output values (aligned to four).
 template <int T>
-__device__ __forceinline__ void store_o(void *o, long long at, float v) {
+__device__ __forceinline__ void store_o4(void *o, long long at, float x, float y, float z, float w) {
   if constexpr (T == ROUGE_B200_T_F32)
-    static_cast<float *>(o)[at] = v;
+    *reinterpret_cast<float4 *>(static_cast<float *>(o) + at) = make_float4(x, y, z, w);
   else if constexpr (T == ROUGE_B200_T_F16)
-    static_cast<uint16_t *>(o)[at] = static_cast<uint16_t>(f16x2_rn(v, 0.0f));
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
+        make_uint2(f16x2_rn(x, y), f16x2_rn(z, w));
   else
-    static_cast<uint16_t *>(o)[at] = static_cast<uint16_t>(bf16x2_rn(v, 0.0f));
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
+        make_uint2(bf16x2_rn(x, y), bf16x2_rn(z, w));
 }
 
 // Warps per block and blocks per SM: 16 warps an SM where a warp's O^T
@@ -189,7 +201,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
   __shared__ long long total_slot[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int gw = blockIdx.x * kWarps + warp;
+  const int gw = warp * gridDim.x + blockIdx.x;  // (few warps: one per SM)
   grid_launch_dependents();
 
   // total work
@@ -208,10 +220,11 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) total += total_slot[i];
   // active warps, and this warp's range of tiles
-  long long active = total / kMinTiles;
+  long long active = total >> kMinTilesLog2;
   active = active < 1 ? 1 : (active > a.warps ? a.warps : active);
-  long long pos = gw < active ? total * gw / active : 0;
-  const long long pos_end = gw < active ? total * (gw + 1) / active : 0;
+  const long long share = divide(total, active), rest = total - share * active;
+  long long pos = gw * share + (gw < rest ? gw : rest);
+  const long long pos_end = gw < active ? pos + share + (gw < rest ? 1 : 0) : pos;
   if (lane < 2) a.desc[2 * gw + lane] = make_int4(0, 0, 0, 0);
   __syncwarp();
   if (pos >= pos_end) return;
@@ -243,6 +256,12 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
   const int stage_sz = stage_bytes(Dh);
   uint8_t *ring = smem + static_cast<size_t>(warp) * S::STAGES * stage_sz;
   const volatile int never = 0;
+  // this lane's copies (see issue)
+  const uint8_t *copy_src = (lane & 6) == 0 ? a.k_codes : (lane & 6) == 2 ? a.v_codes
+                            : (lane & 6) == 4 ? a.k_scales : a.v_scales;
+  const unsigned copy_bytes = 16u * ((lane & 4) ? sbk : cb);
+  const int copy_dst = ((lane & 4) ? 2 * kTile * cb : 0) + ((lane & 2) ? 2 : 0) * copy_bytes +
+                       (lane & 1) * copy_bytes;
   const int k_row = key_of_row(g);                                  // + 8: the lane's other row
   const int v_row[2] = {key_of_row(2 * t), key_of_row(2 * t + 1)};  // + 8: two more
   uint32_t it = 0;  // tiles taken from the ring so far
@@ -256,7 +275,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     }
     // unit and its tiles [u_lo, u_hi) in this warp's range
     const long long in_seq = pos - before;
-    const int unit = static_cast<int>(in_seq / si.tiles);
+    const int unit = static_cast<int>(divide(in_seq, si.tiles));
     const int first = static_cast<int>(in_seq - static_cast<long long>(unit) * si.tiles);
     const int hk = unit % a.Hkv, rt = unit / a.Hkv;
     const long long left = pos_end - pos;
@@ -286,50 +305,44 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     const int t_lo = max(si.lo_tile + first, lo_min / kTile);
     const int t_hi = min(si.lo_tile + last, (hi_max + kTile - 1) / kTile);
 
-    // ---- copies: half tiles of 16 keys, each within one page
+    // ---- copies: half tiles of 16 keys, each within one page. Lane l of the
+    // first eight copies array l / 2 (K codes, V codes, K scales, V scales),
+    // half l % 2.
     const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
-    auto half_page = [&](int half) {  // page of keys [16 * half, +16), -1 if none
+    // first row / 16 of keys [16 * half, +16) in the cache's arrays (below
+    // 2^32: 16 rows take at least 128 bytes of codes), or none
+    constexpr unsigned kNone = 0xFFFFFFFFu;
+    auto half_row = [&](int half) {
       const int key = half * 16;
-      if (key >= hi_max || key + 16 <= lo_min) return -1;  // (no row's keys)
+      if (key >= hi_max || key + 16 <= lo_min) return kNone;  // (no row's keys)
       const int pi = key / a.page;
       const int id = pi < a.max_pages ? __ldg(table + pi) : -1;
       if (id < 0 || id >= a.pages) {
         atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
-        return -1;
+        return kNone;
       }
-      return id;
+      return (static_cast<unsigned>(id) * a.Hkv + hk) * (a.page / 16) + (key - pi * a.page) / 16;
     };
-    int ids = -1, ids_base = -1;  // lane l: page of half tile ids_base + l
+    unsigned rows16 = kNone;       // lane l: half_row(rows_base + l)
+    int rows_base = -1;
     unsigned ok_bits = 0;          // two bits per stage: the halves copied
     auto issue = [&](int tile, uint32_t n) {  // tile into ring slot n % STAGES
       const int h0 = 2 * tile;
-      if (ids_base < 0 || h0 >= ids_base + 32) {
-        ids_base = h0;
-        ids = half_page(h0 + lane);
+      if (rows_base < 0 || h0 >= rows_base + 32) {
+        rows_base = h0;
+        rows16 = half_row(h0 + lane);
       }
-      const int id0 = __shfl_sync(0xffffffffu, ids, h0 - ids_base);
-      const int id1 = __shfl_sync(0xffffffffu, ids, h0 - ids_base + 1);
+      const unsigned row = __shfl_sync(0xffffffffu, rows16, h0 - rows_base + (lane & 1));
+      const unsigned bits = __ballot_sync(0xffffffffu, row != kNone) & 3u;
       const int s = n % S::STAGES;
-      const unsigned bits = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
       ok_bits = (ok_bits & ~(3u << (2 * s))) | (bits << (2 * s));
-      if (lane == 0) {
-        uint8_t *dst = ring + s * stage_sz;
-        const int hb = 16 * (cb + sbk) * 2;  // bytes of one half
-        mbar_arrive_expect_tx(&full[warp][s], static_cast<uint32_t>(hb * ((bits & 1) + (bits >> 1))));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int id = h ? id1 : id0;
-          if (id < 0) continue;
-          const int key = tile * kTile + h * 16;
-          const size_t row = (static_cast<size_t>(id) * a.Hkv + hk) * a.page + key % a.page;
-          bulk_load(dst + h * 16 * cb, a.k_codes + row * cb, 16 * cb, &full[warp][s]);
-          bulk_load(dst + kTile * cb + h * 16 * cb, a.v_codes + row * cb, 16 * cb, &full[warp][s]);
-          bulk_load(dst + 2 * kTile * cb + h * 16 * sbk, a.k_scales + row * sbk, 16 * sbk,
-                    &full[warp][s]);
-          bulk_load(dst + 2 * kTile * cb + kTile * sbk + h * 16 * sbk, a.v_scales + row * sbk,
-                    16 * sbk, &full[warp][s]);
-        }
-      }
+      if (lane == 0)
+        mbar_arrive_expect_tx(&full[warp][s],
+                              static_cast<uint32_t>(32 * (cb + sbk) * ((bits & 1) + (bits >> 1))));
+      __syncwarp();
+      if (lane < 8 && row != kNone)
+        bulk_load(ring + s * stage_sz + copy_dst, copy_src + static_cast<size_t>(row) * copy_bytes,
+                  copy_bytes, &full[warp][s]);
     };
     int ahead = t_lo;
     uint32_t n_issued = it;
@@ -363,9 +376,12 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
         // exponent of the row maximum (0 for an empty or unbounded row)
-        const int e = (m > 0.0f && m < INFINITY) ? ilogbf(m) : 0;
+        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+        if (e == 128) e = 0;             // (infinity or NaN)
+        e = e < -100 ? -100 : e;         // (tiny rows stay tiny)
+        const float down = pow2(-(e / 2)), down2 = pow2(-(e - e / 2));
 #pragma unroll
-        for (int k = 0; k < DT / 4; ++k) v[k] = scalbnf(v[k], -e);
+        for (int k = 0; k < DT / 4; ++k) v[k] = v[k] * down * down2;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -379,7 +395,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
             }
           }
         // (kept positive: a masked score is -inf before it is scaled)
-        const float mine = fmaxf(scalbnf(a.scale * 1.44269504f * gk, e), 1e-37f);
+        const float mine = fmaxf(a.scale * 1.44269504f * gk * pow2(e / 2) * pow2(e - e / 2), 1e-37f);
         mult[j][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
         mult[j][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
       }
@@ -638,20 +654,22 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         if (r >= nrows) continue;
         const float f = whole ? (l > 0.0f || l != l ? gv / l : 0.0f) : 1.0f;
         const int qi = si.q0 + r / a.group, h = hk * a.group + r % a.group;
-        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh;
+        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh + g * (DT / 8);
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+        for (int m = 0; m < kMt; m += 2) {  // values g * DT / 8 + 2m .. + 3
+          if (!FULL && g * (DT / 8) + 2 * m >= Dh) continue;
+          float v[4];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int d = g * (DT / 8) + 2 * m + u;
-            if (!FULL && d >= Dh) continue;
-            float v = o[j][m][2 * u + e];
-            if constexpr (S::SPLIT) v += o[S::NR + j][m][2 * u + e];
-            if (whole)
-              store_o<T>(a.O, at + d, v * f);
-            else
-              part[rr * Dh + d] = v;
+          for (int i = 0; i < 4; ++i) {
+            v[i] = o[j][m + i / 2][2 * (i & 1) + e];
+            if constexpr (S::SPLIT) v[i] += o[S::NR + j][m + i / 2][2 * (i & 1) + e];
           }
+          if (whole)
+            store_o4<T>(a.O, at + 2 * m, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+          else
+            *reinterpret_cast<float4 *>(part + rr * Dh + g * (DT / 8) + 2 * m) =
+                make_float4(v[0], v[1], v[2], v[3]);
+        }
         if (!whole && g == 0) {
           part[S::ROWS * Dh + rr] = mx[j][e];
           part[S::ROWS * (Dh + 1) + rr] = l;
@@ -740,10 +758,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
       const int row = u.z * rows + rr;
       const long long at =
           (static_cast<long long>(q0 + row / a.group) * a.Hq + u.y * a.group + row % a.group) * a.Dh + d;
-      store_o<T>(a.O, at, v.x * f);
-      store_o<T>(a.O, at + 1, v.y * f);
-      store_o<T>(a.O, at + 2, v.z * f);
-      store_o<T>(a.O, at + 3, v.w * f);
+      store_o4<T>(a.O, at, v.x * f, v.y * f, v.z * f, v.w * f);
     }
   }
 }
@@ -764,7 +779,7 @@ int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, i
   const double rts = std::ceil(static_cast<double>(group) * max_q / rows);
   const double tiles = max_kv < kTile ? 1.0 : std::ceil(static_cast<double>(max_kv) / kTile);
   const int cap = current_sm_count() * ctas_of(Dh, nt);
-  const double want = std::ceil(static_cast<double>(B) * Hkv * rts * tiles / kMinTiles / warps);
+  const double want = std::ceil(static_cast<double>(B) * Hkv * rts * tiles / (1 << kMinTilesLog2) / warps);
   return (want < cap ? static_cast<int>(want) : cap) * warps;
 }
 
