@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
                        (lane & 1) * copy_bytes;
   const int k_row = key_of_row(g);                                  // + 8: the lane's other row
   const int v_row[2] = {key_of_row(2 * t), key_of_row(2 * t + 1)};  // + 8: two more
-  uint32_t it = 0;  // tiles taken from the ring so far
+  int s_in = 0, s_out = 0;   // ring slots of the next copy and the next tile
+  uint32_t parity = 0;       // of s_out's barrier
   bool alive = true;
 
   SeqInfo si = seq_info(a, b, S::ROWS);
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     unsigned rows16 = kNone;       // lane l: half_row(rows_base + l)
     int rows_base = -1;
     unsigned ok_bits = 0;          // two bits per stage: the halves copied
-    auto issue = [&](int tile, uint32_t n) {  // tile into ring slot n % STAGES
+    auto issue = [&](int tile) {  // tile into ring slot s_in
       const int h0 = 2 * tile;
       if (rows_base < 0 || h0 >= rows_base + 32) {
         rows_base = h0;
@@ -334,7 +335,8 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
       }
       const unsigned row = __shfl_sync(0xffffffffu, rows16, h0 - rows_base + (lane & 1));
       const unsigned bits = __ballot_sync(0xffffffffu, row != kNone) & 3u;
-      const int s = n % S::STAGES;
+      const int s = s_in;
+      s_in = s == S::STAGES - 1 ? 0 : s + 1;
       ok_bits = (ok_bits & ~(3u << (2 * s))) | (bits << (2 * s));
       if (lane == 0)
         mbar_arrive_expect_tx(&full[warp][s],
@@ -345,8 +347,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
                   copy_bytes, &full[warp][s]);
     };
     int ahead = t_lo;
-    uint32_t n_issued = it;
-    for (; ahead < t_hi && ahead < t_lo + S::STAGES - 1; ++ahead) issue(ahead, n_issued++);
+    for (; ahead < t_hi && ahead < t_lo + S::STAGES - 1; ++ahead) issue(ahead);
 
     // ---- queries as B fragments, scaled to [1, 2) per row
     uint32_t qf[NT][kSteps][2];
@@ -417,18 +418,18 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         sum[j][e] = 0.0f;
       }
 
-    for (int tile = t_lo; tile < t_hi; ++tile, ++it) {
-      if (ahead < t_hi) {
-        issue(ahead, n_issued++);
-        ++ahead;
-      }
-      const int s = it % S::STAGES;
+    int tile = t_lo;
+    for (; tile < t_hi; ++tile) {
+      if (ahead < t_hi) issue(ahead++);
+      const int s = s_out;
       const unsigned ok = (ok_bits >> (2 * s)) & 3u;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][s], (it / S::STAGES) & 1u, &never))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][s], parity, &never))) {
         if (lane == 0) atomicCAS(a.err, 0, ROUGE_B200_ETIMEOUT);
         alive = false;
         break;
       }
+      s_out = s == S::STAGES - 1 ? 0 : s + 1;
+      parity ^= s_out == 0 ? 1u : 0u;
       const uint8_t *kc = ring + s * stage_sz, *vc = kc + kTile * cb;
       const uint8_t *ks = kc + 2 * kTile * cb, *vs = ks + kTile * sbk;
       const int key0 = tile * kTile;
@@ -577,15 +578,37 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
 
       // ---- weighted sums: the lane's keys of weight rows 2t, 2t + 1, 2t + 8,
       // 2t + 9, values d = g * DT / 8 + ...
+      constexpr int kSb = DT == 256 ? 2 : 1;  // scale blocks of the lane's values
+      uint32_t sv[2][4][kSb];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int w = 0; w < kSb; ++w)
+            sv[kb][q][w] = FULL || g * (DT / 8) + 16 * w < Dh
+                               ? vs[(kb * 16 + v_row[q & 1] + (q & 2) * 4) * sbk +
+                                    (DT == 64 ? g / 2 : g * kSb) + w]
+                               : 0u;
+      if (masked) {  // keys of no row: a zero scale, whatever the page holds
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int key = key0 + kb * 16 + v_row[q & 1] + (q & 2) * 4;
+            if (!((ok >> kb) & 1u) || key >= hi_max || key < lo_min) {
+#pragma unroll
+              for (int w = 0; w < kSb; ++w) sv[kb][q][w] = 0u;
+            }
+          }
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        constexpr int kSb = DT == 256 ? 2 : 1;  // scale blocks of the lane's values
-        uint32_t c[4][kVw], sv[4][kSb];
+        uint32_t c[4][kVw], s01 = 0, s23 = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int row = kb * 16 + v_row[q & 1] + (q & 2) * 4;
           const uint8_t *pc = vc + row * cb + g * (DT / 16);
-          const uint8_t *ps = vs + row * sbk + (DT == 64 ? g / 2 : g * kSb);
           if constexpr (FULL && kVw == 2) {
             const uint2 v = *reinterpret_cast<const uint2 *>(pc);
             c[q][0] = v.x; c[q][1] = v.y;
@@ -598,21 +621,14 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
               c[q][w] = FULL || g * (DT / 8) + 8 * w < Dh
                             ? *reinterpret_cast<const uint32_t *>(pc + 4 * w) : 0u;
           }
-#pragma unroll
-          for (int w = 0; w < kSb; ++w)
-            sv[q][w] = FULL || g * (DT / 8) + 16 * w < Dh ? ps[w] : 0u;
-          if (masked) {  // keys of no row: a zero scale, whatever the page holds
-            const int key = key0 + row;
-            if (!((ok >> kb) & 1u) || key >= hi_max || key < lo_min) {
-#pragma unroll
-              for (int w = 0; w < kSb; ++w) sv[q][w] = 0u;
-            }
-          }
         }
 #pragma unroll
         for (int w = 0; w < kVw; ++w) {
-          const uint32_t s01 = e4m3x2_f16x2(sv[0][w * kSb / kVw] | (sv[1][w * kSb / kVw] << 8));
-          const uint32_t s23 = e4m3x2_f16x2(sv[2][w * kSb / kVw] | (sv[3][w * kSb / kVw] << 8));
+          constexpr int kPer = kVw / kSb;  // words of one scale block
+          if (w % kPer == 0) {
+            s01 = e4m3x2_f16x2(sv[kb][0][w / kPer] | (sv[kb][1][w / kPer] << 8));
+            s23 = e4m3x2_f16x2(sv[kb][2][w / kPer] | (sv[kb][3][w / kPer] << 8));
+          }
           constexpr uint32_t kLo = 0x0F0F0F0Fu;
           uint32_t ev01[4], od01[4], ev23[4], od23[4];
           e2m1x8_f16x2((c[0][w] & kLo) | ((c[1][w] << 4) & ~kLo), ev01);
@@ -632,8 +648,11 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
       __syncwarp();  // every lane has read the stage before it is filled again
     }
     if (!alive) {  // the copies still under way land before the block's memory is released
-      for (uint32_t n = it; n < n_issued; ++n)
-        mbar_wait(&full[warp][n % S::STAGES], (n / S::STAGES) & 1u, &never);
+      for (; tile < ahead; ++tile) {
+        mbar_wait(&full[warp][s_out], parity, &never);
+        s_out = s_out == S::STAGES - 1 ? 0 : s_out + 1;
+        parity ^= s_out == 0 ? 1u : 0u;
+      }
       break;
     }
 
