@@ -3,18 +3,21 @@
 //   y = (float)(h / sqrt(sum h^2 / n + eps)) * w      (transformer.cpp:33-40)
 //   codes, scales = per-row int8 (quant_int8.cpp:72-90) or MXFP8 e4m3
 //                   blocks of 32 (narrow.cpp:200-265) of y
-// with the same arithmetic as those steps apart: sum of squares, inverse
-// root and the scaled product in double, so the codes are those of
-// rouge_rmsnorm followed by the quantizer.
+// with the arithmetic of those steps apart: sum of squares and inverse root
+// in double, the scaled product rounded once (norm_value), so the codes are
+// those of rouge_rmsnorm followed by the quantizer.
 //
 // Memory-bound: a row is read once and stays in registers (16 values per
 // thread) over both reductions -- the sum of squares, then the row maximum
-// of y -- and the codes. One to 32 warps share a row, so that 512 to 16384
-// columns fit; longer rows take the looping kernel, which reads h again.
+// of y -- and the codes, while the block's next row is on its way into other
+// registers. One to 32 warps share a row, so that 512 to 16384 columns fit;
+// longer rows take the looping kernel, which reads h again.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <cmath>
 #include <cstdint>
 
 #include "i8code.cuh"
@@ -36,44 +39,55 @@ struct NormArgs {
   void *codes, *scales;
 };
 
-template <int T>
-struct Elem {
-  using type = uint16_t;
-};
-template <>
-struct Elem<ROUGE_B200_T_F32> {
-  using type = float;
-};
-
-// V consecutive elements (V * sizeof(element) bytes, aligned) as f32.
+// V consecutive elements of type T as they lie in memory (8 or 16 bytes).
 template <int T, int V>
-__device__ __forceinline__ void load_vec(const void *base, long long at, float (&v)[V]) {
-  if constexpr (T == ROUGE_B200_T_F32) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const float4 t = *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at + 4 * q);
-      v[4 * q] = t.x; v[4 * q + 1] = t.y; v[4 * q + 2] = t.z; v[4 * q + 3] = t.w;
-    }
-  } else {
-    uint32_t u[V / 2];
-    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-    if constexpr (V == 8) {
-      const uint4 t = *reinterpret_cast<const uint4 *>(p);
-      u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w;
-    } else {
+struct Raw {
+  static constexpr int WORDS = T == ROUGE_B200_T_F32 ? V : V / 2;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const void *base, long long at) {
+    const char *p = static_cast<const char *>(base) + at * (T == ROUGE_B200_T_F32 ? 4 : 2);
+    if constexpr (WORDS == 2) {
       const uint2 t = *reinterpret_cast<const uint2 *>(p);
-      u[0] = t.x; u[1] = t.y;
+      w[0] = t.x; w[1] = t.y;
+    } else {
+      const uint4 t = *reinterpret_cast<const uint4 *>(p);
+      w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
     }
+  }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int q = 0; q < V / 2; ++q) {
-      if constexpr (T == ROUGE_B200_T_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[q]));
+    for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void unpack(float (&v)[V]) const {
+#pragma unroll
+    for (int q = 0; q < WORDS; ++q) {
+      if constexpr (T == ROUGE_B200_T_F32) {
+        v[q] = __uint_as_float(w[q]);
+      } else if constexpr (T == ROUGE_B200_T_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[q]));
         v[2 * q] = f.x; v[2 * q + 1] = f.y;
       } else {
-        v[2 * q] = __uint_as_float(u[q] << 16);
-        v[2 * q + 1] = __uint_as_float(u[q] & 0xFFFF0000u);
+        v[2 * q] = __uint_as_float(w[q] << 16);
+        v[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
       }
     }
+  }
+};
+
+template <int T, int V>
+__device__ __forceinline__ void load_vec(const void *base, long long at, float (&v)[V]) {
+  Raw<T, V> r;
+  r.load(base, at);
+  r.unpack(v);
+}
+
+// The weights of V columns.
+template <int V>
+__device__ __forceinline__ void load_weights(const float *w, int c, float (&v)[V]) {
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    const float4 t = __ldg(reinterpret_cast<const float4 *>(w + c) + q);
+    v[4 * q] = t.x; v[4 * q + 1] = t.y; v[4 * q + 2] = t.z; v[4 * q + 3] = t.w;
   }
 }
 
@@ -111,44 +125,89 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
 }
 
-// Reductions over the WPR warps of a row group; `slot` holds 2 x WPR values
-// of this group, used in turn so that one barrier per reduction is enough
-// (a slot is written again only after the other reduction's barrier).
-template <int WPR, class V, class Op>
-__device__ __forceinline__ V group_reduce(V v, V *slot, int group, int wig, int lane, Op op) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if constexpr (WPR > 1) {
-    if (lane == 0) slot[wig] = v;
-    group_sync(group, WPR * 32);
-    v = slot[0];
-#pragma unroll
-    for (int i = 1; i < WPR; ++i) v = op(v, slot[i]);
-  }
-  return v;
-}
-
-// y of one value: (float)(h * inv), then * w, both rounded (rouge_rmsnorm).
-__device__ __forceinline__ float norm_value(float h, double inv, float w) {
-  return __fmul_rn(__double2float_rn(__dmul_rn(static_cast<double>(h), inv)), w);
-}
-
 __device__ __forceinline__ double norm_inverse(double ss, int n, float eps) {
   return __ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__ddiv_rn(ss, static_cast<double>(n)),
                                              static_cast<double>(eps))));
+}
+
+// The row's inverse root mean square in two floats, hi + lo = the double to
+// 2^-48.
+struct InvRms {
+  float hi, lo;
+};
+__device__ __forceinline__ InvRms split_inverse(double inv) {
+  const float hi = __double2float_rn(inv);
+  // (an infinite or NaN inverse has no low part)
+  const float lo = isinf(hi) || isnan(hi) ? 0.0f : __double2float_rn(__dsub_rn(inv, hi));
+  return InvRms{hi, lo};
+}
+
+// y of one value: h times the inverse rounded once to f32, then times w,
+// rounded (rouge_rmsnorm's arithmetic, whose product is in double). The
+// product is taken in two floats -- p + t with t good to 2^-24 of itself --
+// instead of double, whose conversions run at an eighth of the rate; the
+// rounded sum is the double's but where that lies within 2^-47 of the middle
+// of two floats.
+__device__ __forceinline__ float norm_value(float h, InvRms inv, float w) {
+  const float p = __fmul_rn(h, inv.hi);
+  const float t = __fmaf_rn(h, inv.lo, __fmaf_rn(h, inv.hi, -p));
+  // (an infinite p has a NaN remainder; a remainder below the subnormals is 0)
+  const float y = fabsf(p) < INFINITY ? __fadd_rn(p, t) : p;
+  return __fmul_rn(y, w);
+}
+
+// Scale of an int8 row from the maximum of |y| (quant_int8.cpp:82-84).
+struct RowScale {
+  double inv;
+  float scale, inv_f;
+};
+__device__ __forceinline__ RowScale row_scale(float amax) {
+  const double m = static_cast<double>(amax);
+  RowScale r;
+  r.scale = m > 0.0 ? __double2float_rn(__ddiv_rn(m, 127.0)) : 1.0f;
+  r.inv = __ddiv_rn(1.0, static_cast<double>(r.scale));
+  r.inv_f = __double2float_rn(r.inv);
+  return r;
+}
+
+// A value reduced over the WPR warps of a row group, and what `finish` makes
+// of it, known to all of them: the warps' parts meet in `slot`, the group's
+// first warp finishes (the double divisions are done once) and leaves the
+// result in `out`. Two barriers; slot and out are written again only after
+// every thread has passed another pair.
+template <int WPR, class V, class R, class Op, class Finish>
+__device__ __forceinline__ R group_reduce(V v, V *slot, R *out, int group, int wig, int lane, Op op,
+                                          Finish finish) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (WPR == 1) {
+    return finish(v);
+  } else {
+    if (lane == 0) slot[wig] = v;
+    group_sync(group, WPR * 32);
+    if (wig == 0) {
+      v = slot[lane % WPR];
+#pragma unroll
+      for (int o = WPR / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+      const R r = finish(v);
+      if (lane == 0) *out = r;
+    }
+    group_sync(group, WPR * 32);
+    return *out;
+  }
 }
 
 // Codes of V consecutive values of one row starting at column c. I8: from
 // the row's scale; MX: each block of 32 is V-value lanes next to each other.
 template <int FMT, int V>
 __device__ __forceinline__ void store_codes(const NormArgs &a, int row, int c, const float (&y)[V],
-                                            bool live, double inv, float inv_f, bool exact_row) {
+                                            bool live, const RowScale &rs) {
   uint32_t w[V / 4];
   if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
 #pragma unroll
     for (int q = 0; q < V / 4; ++q)
-      w[q] = encode4_i8_x2(make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]), inv,
-                           inv_f, exact_row);
+      w[q] = encode4_i8_x2(make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]), rs.inv,
+                           rs.inv_f, isinf(rs.inv_f));
   } else {
     float m = 0.0f;
 #pragma unroll
@@ -172,85 +231,87 @@ __device__ __forceinline__ void store_codes(const NormArgs &a, int row, int c, c
     *reinterpret_cast<uint32_t *>(out) = w[0];
 }
 
-// Scale of an int8 row from the maximum of |y| (quant_int8.cpp:82-84).
-__device__ __forceinline__ float row_scale(float amax) {
-  const double m = static_cast<double>(amax);
-  return m > 0.0 ? __double2float_rn(__ddiv_rn(m, 127.0)) : 1.0f;
-}
-
-template <int T, int V, int FMT, int WPR>
+template <int T, int V, int FMT, int WPR, bool RES>
 __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
     norm_quant_kernel(const NormArgs a) {
   constexpr int kWarps = WPR > 8 ? WPR : 8, kGroups = kWarps / WPR, kNv = kPerThread / V;
   __shared__ double sum_slot[kWarps];
   __shared__ float max_slot[kWarps];
+  __shared__ InvRms rms_out[kGroups];
+  __shared__ RowScale scale_out[kGroups];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = warp / WPR, wig = warp % WPR;
-  const int tig = wig * 32 + lane;  // thread within the row group
-  for (int row = blockIdx.x * kGroups + group; row < a.rows; row += gridDim.x * kGroups) {
+  const int c0 = (wig * 32 + lane) * V;  // first column; the next kNv - 1 are WPR * 32 * V apart
+  constexpr int kStep = WPR * 32 * V;
+  Raw<T, V> xr[kNv], rr[RES ? kNv : 1];
+  auto fetch = [&](int row) {
+#pragma unroll
+    for (int i = 0; i < kNv; ++i) {
+      const int c = c0 + i * kStep;
+      if (c < a.cols) {
+        xr[i].load(a.x, row * a.ldx + c);
+        if constexpr (RES) rr[i].load(a.r, row * a.ldr + c);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kNv; ++i) {  // (columns past the row stay zeros)
+    xr[i].zero();
+    if constexpr (RES) rr[i].zero();
+  }
+  int row = blockIdx.x * kGroups + group;
+  if (row < a.rows) fetch(row);
+  for (; row < a.rows; row += gridDim.x * kGroups) {
     float h[kNv][V];
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < kNv; ++i) {
-      const int c = (i * WPR * 32 + tig) * V;
-      if (c < a.cols) {
-        load_vec<T, V>(a.x, row * a.ldx + c, h[i]);
-        if (a.r) {
-          float t[V];
-          load_vec<T, V>(a.r, row * a.ldr + c, t);
+      const int c = c0 + i * kStep;
+      xr[i].unpack(h[i]);
+      if constexpr (RES) {
+        float t[V];
+        rr[i].unpack(t);
 #pragma unroll
-          for (int j = 0; j < V; ++j) h[i][j] = __fadd_rn(h[i][j], t[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = 0.0f;
+        for (int j = 0; j < V; ++j) h[i][j] = __fadd_rn(h[i][j], t[j]);
+        if (c < a.cols) round_store<T, V>(a.h, row * a.ldh + c, h[i]);
       }
     }
+    // the next row's loads run under this row's reductions and codes
+    const int next = row + gridDim.x * kGroups;
+    if (next < a.rows) fetch(next);
 #pragma unroll
-    for (int i = 0; i < kNv; ++i) {
-      const int c = (i * WPR * 32 + tig) * V;
-      if (a.r && c < a.cols) round_store<T, V>(a.h, row * a.ldh + c, h[i]);
+    for (int i = 0; i < kNv; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = __fma_rn(static_cast<double>(h[i][j]), h[i][j], ss);
-    }
-    ss = group_reduce<WPR>(ss, sum_slot + group * WPR, group, wig, lane,
-                           [](double p, double q) { return __dadd_rn(p, q); });
-    const double inv_rms = norm_inverse(ss, a.cols, a.eps);
+    const InvRms inv = group_reduce<WPR>(
+        ss, sum_slot + group * WPR, rms_out + group, group, wig, lane,
+        [](double p, double q) { return __dadd_rn(p, q); },
+        [&](double v) { return split_inverse(norm_inverse(v, a.cols, a.eps)); });
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kNv; ++i) {
-      const int c = (i * WPR * 32 + tig) * V;
-      float wv[V];
+      const int c = c0 + i * kStep;
       if (c < a.cols) {
-        load_vec<ROUGE_B200_T_F32, V>(a.w, c, wv);
-      } else {
+        float wv[V];
+        load_weights<V>(a.w, c, wv);
 #pragma unroll
-        for (int j = 0; j < V; ++j) wv[j] = 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        h[i][j] = c < a.cols ? norm_value(h[i][j], inv_rms, wv[j]) : 0.0f;
-        amax = fmaxf(amax, fabsf(h[i][j]));
+        for (int j = 0; j < V; ++j) {
+          h[i][j] = norm_value(h[i][j], inv, wv[j]);
+          amax = fmaxf(amax, fabsf(h[i][j]));
+        }
       }
     }
-    double inv = 0.0;
-    float inv_f = 0.0f;
-    bool exact_row = false;
+    RowScale rs{};
     if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
-      amax = group_reduce<WPR>(amax, max_slot + group * WPR, group, wig, lane,
-                               [](float p, float q) { return fmaxf(p, q); });
-      const float s = row_scale(amax);
-      inv = __ddiv_rn(1.0, static_cast<double>(s));
-      inv_f = __double2float_rn(inv);
-      exact_row = isinf(inv_f);
-      if (tig == 0) static_cast<float *>(a.scales)[row] = s;
-    } else if constexpr (WPR > 1) {
-      group_sync(group, WPR * 32);  // (the sum's slots are read before the next row writes them)
+      rs = group_reduce<WPR>(amax, max_slot + group * WPR, scale_out + group, group, wig, lane,
+                             [](float p, float q) { return fmaxf(p, q); },
+                             [](float v) { return row_scale(v); });
+      if (wig == 0 && lane == 0) static_cast<float *>(a.scales)[row] = rs.scale;
     }
 #pragma unroll
     for (int i = 0; i < kNv; ++i) {
-      const int c = (i * WPR * 32 + tig) * V;
-      store_codes<FMT, V>(a, row, c, h[i], c < a.cols, inv, inv_f, exact_row);
+      const int c = c0 + i * kStep;
+      store_codes<FMT, V>(a, row, c, h[i], c < a.cols, rs);
     }
   }
 }
@@ -261,6 +322,8 @@ template <int T, int V, int FMT>
 __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a) {
   __shared__ double sum_slot[32];
   __shared__ float max_slot[32];
+  __shared__ InvRms rms_out;
+  __shared__ RowScale scale_out;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const void *src = a.r ? a.h : a.x;
   const long long lds = a.r ? a.ldh : a.ldx;
@@ -279,19 +342,17 @@ __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = __fma_rn(static_cast<double>(h[j]), h[j], ss);
     }
-    ss = group_reduce<32>(ss, sum_slot, 0, warp, lane,
-                          [](double p, double q) { return __dadd_rn(p, q); });
-    const double inv_rms = norm_inverse(ss, a.cols, a.eps);
+    const InvRms inv = group_reduce<32>(
+        ss, sum_slot, &rms_out, 0, warp, lane, [](double p, double q) { return __dadd_rn(p, q); },
+        [&](double v) { return split_inverse(norm_inverse(v, a.cols, a.eps)); });
     auto values = [&](int c, float (&y)[V]) {
       float wv[V];
       load_vec<T, V>(src, row * lds + c, y);
-      load_vec<ROUGE_B200_T_F32, V>(a.w, c, wv);
+      load_weights<V>(a.w, c, wv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = norm_value(y[j], inv_rms, wv[j]);
+      for (int j = 0; j < V; ++j) y[j] = norm_value(y[j], inv, wv[j]);
     };
-    double inv = 0.0;
-    float inv_f = 0.0f;
-    bool exact_row = false;
+    RowScale rs{};
     if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
       float amax = 0.0f;
       for (int c = threadIdx.x * V; c < a.cols; c += 1024 * V) {
@@ -300,19 +361,14 @@ __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(y[j]));
       }
-      amax = group_reduce<32>(amax, max_slot, 0, warp, lane,
-                              [](float p, float q) { return fmaxf(p, q); });
-      const float s = row_scale(amax);
-      inv = __ddiv_rn(1.0, static_cast<double>(s));
-      inv_f = __double2float_rn(inv);
-      exact_row = isinf(inv_f);
-      if (threadIdx.x == 0) static_cast<float *>(a.scales)[row] = s;
-    } else {
-      __syncthreads();
+      rs = group_reduce<32>(amax, max_slot, &scale_out, 0, warp, lane,
+                            [](float p, float q) { return fmaxf(p, q); },
+                            [](float v) { return row_scale(v); });
+      if (threadIdx.x == 0) static_cast<float *>(a.scales)[row] = rs.scale;
     }
     // (whole warps: a block's lanes take part in its shuffles)
-    for (int c0 = 0; c0 < a.cols; c0 += 1024 * V) {
-      const int c = c0 + threadIdx.x * V;
+    for (int c1 = 0; c1 < a.cols; c1 += 1024 * V) {
+      const int c = c1 + threadIdx.x * V;
       float y[V];
       if (c < a.cols) {
         values(c, y);
@@ -320,19 +376,32 @@ __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) y[j] = 0.0f;
       }
-      store_codes<FMT, V>(a, row, c, y, c < a.cols, inv, inv_f, exact_row);
+      store_codes<FMT, V>(a, row, c, y, c < a.cols, rs);
     }
   }
+}
+
+template <class Kernel>
+int launch_rows(Kernel kernel, const NormArgs &a, int threads, int groups, std::atomic<int> &per_sm,
+                cudaStream_t st) {
+  int n = per_sm.load();
+  if (n == 0) {  // resident blocks per SM: a block takes row after row
+    const int s = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0));
+    if (s != ROUGE_B200_OK) return s;
+    per_sm.store(n = n < 1 ? 1 : n);
+  }
+  const long long want = (static_cast<long long>(a.rows) + groups - 1) / groups;
+  const long long cap = static_cast<long long>(current_sm_count()) * n;
+  kernel<<<static_cast<unsigned>(want < cap ? want : cap), threads, 0, st>>>(a);
+  return cuda_status(cudaGetLastError());
 }
 
 template <int T, int V, int FMT, int WPR>
 int launch_wpr(const NormArgs &a, cudaStream_t st) {
   constexpr int kThreads = WPR > 8 ? WPR * 32 : 256, kGroups = kThreads / 32 / WPR;
-  const long long want = (static_cast<long long>(a.rows) + kGroups - 1) / kGroups;
-  const long long cap = static_cast<long long>(current_sm_count()) * (2048 / kThreads);
-  norm_quant_kernel<T, V, FMT, WPR>
-      <<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(a);
-  return cuda_status(cudaGetLastError());
+  static std::atomic<int> with{0}, without{0};
+  return a.r ? launch_rows(norm_quant_kernel<T, V, FMT, WPR, true>, a, kThreads, kGroups, with, st)
+             : launch_rows(norm_quant_kernel<T, V, FMT, WPR, false>, a, kThreads, kGroups, without, st);
 }
 
 // Warps per row: the fewest whose registers hold it.
