@@ -12,12 +12,29 @@
 
 #include "kv4.cuh"
 #include "narrow.cuh"
+#include "ptx.cuh"
 #include "x86fp.cuh"
 
 namespace rb200 {
 namespace {
 
 constexpr int kThreads = 256;
+
+// Division of n < 2^31 by a value fixed on the host (32-bit sizes): one
+// high product and a shift, with the rounded-up reciprocal
+// mul = ceil(2^(32 + shift) / d), shift = ceil(log2 d) - 1, whose error
+// n (mul d - 2^(32 + shift)) / (d 2^(32 + shift)) stays below 1 / d.
+struct Divisor {
+  unsigned d, mul, shift;
+  Divisor(unsigned v = 1) : d(v), mul(0), shift(0) {
+    if (v == 1) return;
+    while ((2u << shift) < v) ++shift;
+    mul = static_cast<unsigned>(((1ull << (32 + shift)) + v - 1) / v);
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const {
+    return d == 1 ? n : __umulhi(n, mul) >> shift;
+  }
+};
 
 struct KvArgs {
   uint8_t *codes[2], *scales[2];
@@ -26,8 +43,9 @@ struct KvArgs {
   void *dst[2];
   long long ld[2];
   int page, Hkv, nblk;  // nblk = Dh / 16
+  Divisor by_nblk, by_heads, by_page;
   int total_slots;
-  long long items;      // T * Hkv * nblk
+  unsigned items;       // tokens * Hkv * nblk of this launch
   const int *slots;
   int *err;
 };
@@ -76,43 +94,48 @@ __device__ __forceinline__ void store16(void *p, long long at, const float (&v)[
 }
 
 // Where item i (token, head, block) lies: false for a skipped token.
-__device__ __forceinline__ bool locate(const KvArgs &a, long long i, int &head, long long &el,
+__device__ __forceinline__ bool locate(const KvArgs &a, unsigned i, int &head, long long &el,
                                        int which, size_t &blk_at) {
-  const int blk = static_cast<int>(i % a.nblk);
-  const long long th = i / a.nblk;
-  head = static_cast<int>(th % a.Hkv);
-  const long long t = th / a.Hkv;
+  const unsigned th = a.by_nblk.div(i), blk = i - th * a.nblk;
+  const unsigned t = a.by_heads.div(th);
+  head = static_cast<int>(th - t * a.Hkv);
   const int slot = __ldg(a.slots + t);
   if (slot < 0) return false;
   if (slot >= a.total_slots) {
     atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
     return false;
   }
-  el = t * a.ld[which] + (static_cast<long long>(head) * a.nblk + blk) * 16;
-  const int p = slot / a.page, at = slot - p * a.page;
+  el = t * a.ld[which] + static_cast<long long>(head * a.nblk + static_cast<int>(blk)) * 16;
+  const int p = a.by_page.div(slot), at = slot - p * a.page;
   blk_at = ((static_cast<size_t>(p) * a.Hkv + head) * a.page + at) * a.nblk + blk;
   return true;
 }
 
-// x / step for a code's border test, correctly rounded: one Newton step on
-// the product with the reciprocal, whose residual is exact while nothing
-// under- or overflows (step between 2^-100 and 2^100); a quotient that is
-// exactly a border between two codes is then met exactly.
-__device__ __forceinline__ float quotient(float x, float step, float inv, bool plain) {
-  if (plain) return __fdiv_rn(x, step);
-  const float q = __fmul_rn(x, inv);
-  const float r = __fmaf_rn(-q, step, x);
-  return fabsf(q) < 8.0f ? __fmaf_rn(r, inv, q) : q;  // (6 and more saturate; NaN and Inf stay)
+// Quotients x / step for the codes' border tests, correctly rounded: one
+// Newton step on the product with the reciprocal, whose residual is exact
+// while nothing under- or overflows; a quotient that is exactly a border
+// between two codes is then met exactly.
+__device__ __forceinline__ void quotients(float &x, float &y, float step, float inv) {
+  float q0, q1, r0, r1;
+  mul2(q0, q1, x, y, inv);
+  fma2(r0, r1, q0, q1, -step, x, y);
+  fma2(x, y, r0, r1, inv, q0, q1);
 }
 
-// -0.25 <= v <= 0 codes +0 (the hardware keeps the sign of a zero).
-__device__ __forceinline__ float drop_sign(float v) { return (v >= -0.25f && v <= 0.0f) ? 0.0f : v; }
+// The same for one value of a block that holds an infinity or a NaN, or whose
+// step is extreme (infinities divide to infinities, NaN stays).
+__device__ __forceinline__ float quotient_any(float x, float step) { return __fdiv_rn(x, step); }
+
+// Clears the sign of zero codes (the hardware keeps it; eight nibbles).
+__device__ __forceinline__ uint32_t unsigned_zeros(uint32_t w) {
+  const uint32_t mag = w & 0x77777777u;
+  return mag | (w & (mag + 0x77777777u) & 0x88888888u);
+}
 
 template <int T>
 __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
   const int which = blockIdx.y;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < a.items;
-       i += static_cast<long long>(gridDim.x) * kThreads) {
+  for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < a.items; i += gridDim.x * kThreads) {
     int head;
     long long el;
     size_t at;
@@ -122,18 +145,29 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
     const float g = a.gs[which] ? __ldg(a.gs[which] + head) : 1.0f;
     float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = fmaxf(m, fabsf(v[j]));
+    for (int j = 0; j < 16; ++j) m = max_nan(m, fabsf(v[j]));
+    const bool odd = !(m < INFINITY);
+    if (m != m) {  // the maximum of the others
+      m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) m = fmaxf(m, fabsf(v[j]));
+    }
     const uint32_t sc = cvt_pair_e4m3(__fdiv_rn(m, __fmul_rn(6.0f, g)), 0.0f) & 0xFFu;
     const uint32_t sh = e4m3x2_f16x2(sc);
     const float step = __fmul_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(sh))), g);
     uint2 w = make_uint2(0u, 0u);
     if (step > 0.0f) {
-      const bool plain = !(step > 7.9e-31f && step < 1.2e30f);
-      const float inv = __fdiv_rn(1.0f, step);
+      if (odd || !(step > 7.9e-31f && step < 1.2e30f)) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = drop_sign(quotient(v[j], step, inv, plain));
-      w.x = cvt4_e2m1(v[0], v[1], v[2], v[3]) | (cvt4_e2m1(v[4], v[5], v[6], v[7]) << 16);
-      w.y = cvt4_e2m1(v[8], v[9], v[10], v[11]) | (cvt4_e2m1(v[12], v[13], v[14], v[15]) << 16);
+        for (int j = 0; j < 16; ++j) v[j] = quotient_any(v[j], step);
+      } else {
+        const float inv = __fdiv_rn(1.0f, step);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) quotients(v[j], v[j + 1], step, inv);
+      }
+      w.x = unsigned_zeros(cvt4_e2m1(v[0], v[1], v[2], v[3]) | (cvt4_e2m1(v[4], v[5], v[6], v[7]) << 16));
+      w.y = unsigned_zeros(cvt4_e2m1(v[8], v[9], v[10], v[11]) |
+                           (cvt4_e2m1(v[12], v[13], v[14], v[15]) << 16));
     }
     reinterpret_cast<uint2 *>(a.codes[which])[at] = w;
     a.scales[which][at] = static_cast<uint8_t>(sc);
@@ -143,8 +177,7 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
 template <int T>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const KvArgs a) {
   const int which = blockIdx.y;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < a.items;
-       i += static_cast<long long>(gridDim.x) * kThreads) {
+  for (unsigned i = blockIdx.x * kThreads + threadIdx.x; i < a.items; i += gridDim.x * kThreads) {
     int head;
     long long el;
     size_t at;
@@ -188,16 +221,35 @@ int prepare(const RougeB200KV4 *c, const void *K, long long ldk, const void *V, 
   a.page = c->page;
   a.Hkv = c->Hkv;
   a.nblk = c->Dh / 16;
+  a.by_nblk = Divisor(a.nblk);
+  a.by_heads = Divisor(a.Hkv);
+  a.by_page = Divisor(a.page);
   a.total_slots = c->pages * c->page;
-  a.items = static_cast<long long>(T) * c->Hkv * a.nblk;
   a.slots = slots;
   return ROUGE_B200_OK;
 }
 
-dim3 grid_of(const KvArgs &a) {
-  const long long want = (a.items + kThreads - 1) / kThreads;
+// Launches `kernel` over the tokens, at most 2^30 items at a time.
+template <class Kernel>
+int launch_tokens(Kernel kernel, KvArgs a, int T, int esize, cudaStream_t st) {
+  const int per_token = a.Hkv * a.nblk;
+  const int step = per_token < (1 << 30) ? (1 << 30) / per_token : 1;
   const long long cap = static_cast<long long>(current_sm_count()) * 8;
-  return dim3(static_cast<unsigned>(want < cap ? want : cap), 2);
+  for (int t0 = 0; t0 < T; t0 += step) {
+    const int n = T - t0 < step ? T - t0 : step;
+    a.items = static_cast<unsigned>(n) * per_token;
+    const long long want = (static_cast<long long>(a.items) + kThreads - 1) / kThreads;
+    kernel<<<dim3(static_cast<unsigned>(want < cap ? want : cap), 2), kThreads, 0, st>>>(a);
+    const int s = cuda_status(cudaGetLastError());
+    if (s != ROUGE_B200_OK || T - t0 <= step) return s;
+    a.slots += n;
+    for (int w = 0; w < 2; ++w) {
+      const long long bytes = n * a.ld[w] * esize;
+      if (a.src[w]) a.src[w] = static_cast<const uint8_t *>(a.src[w]) + bytes;
+      if (a.dst[w]) a.dst[w] = static_cast<uint8_t *>(a.dst[w]) + bytes;
+    }
+  }
+  return ROUGE_B200_OK;
 }
 
 }  // namespace
@@ -220,11 +272,10 @@ int rouge_b200_kv4_write(const RougeB200KV4 *cache, const void *K, long long ldk
   if (!a.err) return set_status(ROUGE_B200_ENOMEM);
   cudaStream_t st = as_stream(stream);
   switch (type) {
-    case ROUGE_B200_T_F32: kv4_write_kernel<ROUGE_B200_T_F32><<<grid_of(a), kThreads, 0, st>>>(a); break;
-    case ROUGE_B200_T_F16: kv4_write_kernel<ROUGE_B200_T_F16><<<grid_of(a), kThreads, 0, st>>>(a); break;
-    default: kv4_write_kernel<ROUGE_B200_T_BF16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    case ROUGE_B200_T_F32: return launch_tokens(kv4_write_kernel<ROUGE_B200_T_F32>, a, T, 4, st);
+    case ROUGE_B200_T_F16: return launch_tokens(kv4_write_kernel<ROUGE_B200_T_F16>, a, T, 2, st);
+    default: return launch_tokens(kv4_write_kernel<ROUGE_B200_T_BF16>, a, T, 2, st);
   }
-  return cuda_status(cudaGetLastError());
 }
 
 int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void *V, long long ldv,
@@ -240,11 +291,10 @@ int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void 
   if (!a.err) return set_status(ROUGE_B200_ENOMEM);
   cudaStream_t st = as_stream(stream);
   switch (type) {
-    case ROUGE_B200_T_F32: kv4_read_kernel<ROUGE_B200_T_F32><<<grid_of(a), kThreads, 0, st>>>(a); break;
-    case ROUGE_B200_T_F16: kv4_read_kernel<ROUGE_B200_T_F16><<<grid_of(a), kThreads, 0, st>>>(a); break;
-    default: kv4_read_kernel<ROUGE_B200_T_BF16><<<grid_of(a), kThreads, 0, st>>>(a); break;
+    case ROUGE_B200_T_F32: return launch_tokens(kv4_read_kernel<ROUGE_B200_T_F32>, a, T, 4, st);
+    case ROUGE_B200_T_F16: return launch_tokens(kv4_read_kernel<ROUGE_B200_T_F16>, a, T, 2, st);
+    default: return launch_tokens(kv4_read_kernel<ROUGE_B200_T_BF16>, a, T, 2, st);
   }
-  return cuda_status(cudaGetLastError());
 }
 
 }  // extern "C"

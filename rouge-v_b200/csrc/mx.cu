@@ -93,12 +93,6 @@ __global__ void __launch_bounds__(kMxThreads, 8)
   }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // e2m1 input fix: the reference encodes magnitudes in (0, 0.25) as +0, the
 // hardware as a signed zero; zeroing the negative ones first makes them
 // agree (-0.25 and -0 keep their sign in both).

@@ -213,6 +213,12 @@ __device__ __forceinline__ uint32_t cvt4_e2m1(float x0, float x1, float x2, floa
       : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
   return r;
 }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 #endif
 
 }  // namespace rb200
