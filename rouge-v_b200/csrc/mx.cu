@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kMxThreads, 8)
         w = encode_e2m1(__fmul_rn(v[u].x, inv)) | (encode_e2m1(__fmul_rn(v[u].y, inv)) << 8) |
             (encode_e2m1(__fmul_rn(v[u].z, inv)) << 16) | (encode_e2m1(__fmul_rn(v[u].w, inv)) << 24);
       } else {
-        w = mx_encode4_f8<ID>(v[u], inv);
+        const float sum = (v[u].x + v[u].y) + (v[u].z + v[u].w);  // (NaN where one of them is)
+        w = mx_encode4_f8<ID>(v[u], inv, sum != sum);
       }
       store4(codes, blk * 32 + sub * 4, n, vec_out, w);
     }

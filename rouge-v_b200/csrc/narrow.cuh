@@ -183,22 +183,30 @@ __device__ __forceinline__ uint32_t encode_e2m1(float v) {
 // out of reach). The hardware conversion equals the reference except for
 // NaN (sign kept by the reference) and for nonzero magnitudes below half
 // the smallest subnormal, which the hardware rounds to a signed zero and
-// the reference to +0. Both show cheaply per group of four: a NaN makes
-// the sum NaN, a signed zero is a 0x80 byte; such groups take the exact
-// path (x86 products, the reference encoder).
+// the reference to +0. With nan set (some value may be one) the group takes
+// the exact path: x86 products, the reference encoder; a signed zero is a
+// 0x80 byte, cleared where its value is neither zero nor exactly half the
+// smallest subnormal.
 template <int ID>
-__device__ __forceinline__ uint32_t mx_encode4_f8(float4 x, float inv) {
-  const float sum = (x.x + x.y) + (x.z + x.w);
-  const uint32_t lo = ID == kE4M3 ? cvt_pair_e4m3(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv))
-                                  : cvt_pair_e5m2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
-  const uint32_t hi = ID == kE4M3 ? cvt_pair_e4m3(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv))
-                                  : cvt_pair_e5m2(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
-  const uint32_t w = lo | (hi << 16);
-  if (sum == sum && __vcmpeq4(w, 0x80808080u) == 0u) return w;
-  return narrow_encode(x86_mul(x.x, inv), ID, false) |
-         (narrow_encode(x86_mul(x.y, inv), ID, false) << 8) |
-         (narrow_encode(x86_mul(x.z, inv), ID, false) << 16) |
-         (narrow_encode(x86_mul(x.w, inv), ID, false) << 24);
+__device__ __forceinline__ uint32_t mx_encode4_f8(float4 x, float inv, bool nan) {
+  const float y[4] = {__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv),
+                      __fmul_rn(x.w, inv)};
+  const uint32_t lo = ID == kE4M3 ? cvt_pair_e4m3(y[0], y[1]) : cvt_pair_e5m2(y[0], y[1]);
+  const uint32_t hi = ID == kE4M3 ? cvt_pair_e4m3(y[2], y[3]) : cvt_pair_e5m2(y[2], y[3]);
+  uint32_t w = lo | (hi << 16);
+  if (nan)
+    return narrow_encode(x86_mul(x.x, inv), ID, false) |
+           (narrow_encode(x86_mul(x.y, inv), ID, false) << 8) |
+           (narrow_encode(x86_mul(x.z, inv), ID, false) << 16) |
+           (narrow_encode(x86_mul(x.w, inv), ID, false) << 24);
+  const uint32_t z = w ^ 0x80808080u;
+  if ((z - 0x01010101u) & ~z & 0x80808080u) {  // some byte is 0x80
+    constexpr float kTiny = ID == kE4M3 ? 0.0009765625f : 7.62939453125e-06f;  // 2^-10, 2^-17
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (((w >> (8 * i)) & 0xFFu) == 0x80u && y[i] < 0.0f && y[i] > -kTiny) w &= ~(0xFFu << (8 * i));
+  }
+  return w;
 }
 
 // Four e2m1 codes (RNE, satfinite) from the hardware conversion, one per

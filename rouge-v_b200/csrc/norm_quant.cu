@@ -27,7 +27,10 @@
 namespace rb200 {
 namespace {
 
-constexpr int kPerThread = 16;  // row values a thread holds
+// Row values a thread holds. (32 of a 16-bit row halve the share of the
+// reductions, about 90 instructions a row, but leave half the threads: 8191 x
+// 8192 bf16 to MXFP8 took 104 us with 32, 86 with 16.)
+constexpr int kPerThread = 16;
 
 struct NormArgs {
   const void *x, *r;
@@ -35,6 +38,7 @@ struct NormArgs {
   const float *w;
   float eps;
   int rows, cols;
+  double by_cols;  // 1 / cols
   void *h;
   void *codes, *scales;
 };
@@ -57,6 +61,28 @@ struct Raw {
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+  }
+  // this += o, rounded to the type (the 16-bit types' packed additions round
+  // the exact sum once; so does the f32 sum rounded to 16 bits, since a sum
+  // too long for f32 is far from the middle of two 16-bit values)
+  __device__ __forceinline__ void add(const Raw &o) {
+#pragma unroll
+    for (int q = 0; q < WORDS; ++q) {
+      if constexpr (T == ROUGE_B200_T_F32) {
+        w[q] = __float_as_uint(__fadd_rn(__uint_as_float(w[q]), __uint_as_float(o.w[q])));
+      } else if constexpr (T == ROUGE_B200_T_F16) {
+        asm("add.rn.f16x2 %0, %0, %1;" : "+r"(w[q]) : "r"(o.w[q]));
+      } else {
+        asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(w[q]) : "r"(o.w[q]));
+      }
+    }
+  }
+  __device__ __forceinline__ void store(void *base, long long at) const {
+    char *p = static_cast<char *>(base) + at * (T == ROUGE_B200_T_F32 ? 4 : 2);
+    if constexpr (WORDS == 2)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   __device__ __forceinline__ void unpack(float (&v)[V]) const {
 #pragma unroll
@@ -91,110 +117,100 @@ __device__ __forceinline__ void load_weights(const float *w, int c, float (&v)[V
   }
 }
 
-// Rounds v to the element type (v then holds the rounded values) and stores.
-template <int T, int V>
-__device__ __forceinline__ void round_store(void *base, long long at, float (&v)[V]) {
-  if constexpr (T == ROUGE_B200_T_F32) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q)
-      *reinterpret_cast<float4 *>(static_cast<float *>(base) + at + 4 * q) =
-          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  } else {
-    uint32_t u[V / 2];
-#pragma unroll
-    for (int q = 0; q < V / 2; ++q) {
-      if constexpr (T == ROUGE_B200_T_F16) {
-        u[q] = f16x2_rn(v[2 * q], v[2 * q + 1]);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[q]));
-        v[2 * q] = f.x; v[2 * q + 1] = f.y;
-      } else {
-        u[q] = bf16x2_rn(v[2 * q], v[2 * q + 1]);
-        v[2 * q] = __uint_as_float(u[q] << 16);
-        v[2 * q + 1] = __uint_as_float(u[q] & 0xFFFF0000u);
-      }
-    }
-    uint16_t *p = static_cast<uint16_t *>(base) + at;
-    if constexpr (V == 8)
-      *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-    else
-      *reinterpret_cast<uint2 *>(p) = make_uint2(u[0], u[1]);
-  }
-}
-
 __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
 }
 
-__device__ __forceinline__ double norm_inverse(double ss, int n, float eps) {
-  return __ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__ddiv_rn(ss, static_cast<double>(n)),
-                                             static_cast<double>(eps))));
-}
-
-// The row's inverse root mean square in two floats, hi + lo = the double to
-// 2^-48.
+// The row's inverse root mean square: the double, and its two leading floats
+// (hi + lo = the double to 2^-48; hi infinite where the double is too large).
 struct InvRms {
+  double full;
   float hi, lo;
 };
-__device__ __forceinline__ InvRms split_inverse(double inv) {
-  const float hi = __double2float_rn(inv);
-  // (an infinite or NaN inverse has no low part)
-  const float lo = isinf(hi) || isnan(hi) ? 0.0f : __double2float_rn(__dsub_rn(inv, hi));
-  return InvRms{hi, lo};
-}
 
-// y of one value: h times the inverse rounded once to f32, then times w,
-// rounded (rouge_rmsnorm's arithmetic, whose product is in double). The
-// product is taken in two floats -- p + t with t good to 2^-24 of itself --
-// instead of double, whose conversions run at an eighth of the rate; the
-// rounded sum is the double's but where that lies within 2^-47 of the middle
-// of two floats.
-__device__ __forceinline__ float norm_value(float h, InvRms inv, float w) {
-  const float p = __fmul_rn(h, inv.hi);
-  const float t = __fmaf_rn(h, inv.lo, __fmaf_rn(h, inv.hi, -p));
-  // (an infinite p has a NaN remainder; a remainder below the subnormals is 0)
-  const float y = fabsf(p) < INFINITY ? __fadd_rn(p, t) : p;
-  return __fmul_rn(y, w);
-}
-
-// Scale of an int8 row from the maximum of |y| (quant_int8.cpp:82-84).
-struct RowScale {
-  double inv;
-  float scale, inv_f;
-};
-__device__ __forceinline__ RowScale row_scale(float amax) {
-  const double m = static_cast<double>(amax);
-  RowScale r;
-  r.scale = m > 0.0 ? __double2float_rn(__ddiv_rn(m, 127.0)) : 1.0f;
-  r.inv = __ddiv_rn(1.0, static_cast<double>(r.scale));
-  r.inv_f = __double2float_rn(r.inv);
+// 1 / sqrt(ss / n + eps) to double accuracy: two Newton steps from the f32
+// approximation (2^-22, 2^-43, 2^-53), in a chain a third as long as double
+// division, root and division; those serve for values out of f32's range.
+__device__ __forceinline__ InvRms inverse_rms(double ss, double by_n, float eps) {
+  const double v = __dadd_rn(__dmul_rn(ss, by_n), static_cast<double>(eps));
+  InvRms r;
+  if (v > 1e-30 && v < 1e30) {
+    double y = static_cast<double>(rsqrtf(__double2float_rn(v)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const double e = __fma_rn(-__dmul_rn(v, y), y, 1.0);  // 1 - v y^2
+      y = __fma_rn(__dmul_rn(0.5, y), e, y);
+    }
+    r.full = y;
+  } else {
+    r.full = __ddiv_rn(1.0, __dsqrt_rn(v));
+  }
+  r.hi = __double2float_rn(r.full);
+  r.lo = __double2float_rn(__dsub_rn(r.full, static_cast<double>(r.hi)));
   return r;
 }
 
-// A value reduced over the WPR warps of a row group, and what `finish` makes
-// of it, known to all of them: the warps' parts meet in `slot`, the group's
-// first warp finishes (the double divisions are done once) and leaves the
-// result in `out`. Two barriers; slot and out are written again only after
-// every thread has passed another pair.
-template <int WPR, class V, class R, class Op, class Finish>
-__device__ __forceinline__ R group_reduce(V v, V *slot, R *out, int group, int wig, int lane, Op op,
-                                          Finish finish) {
+// y of V values in place: h times the inverse rounded once to f32, then
+// times w, rounded (rouge_rmsnorm's arithmetic, whose product is in double).
+// The product is taken in two floats -- p + t with t good to 2^-24 of itself
+// -- instead of double, whose conversions run at an eighth of the rate; the
+// rounded sum is the double's but where that lies within 2^-47 of the middle
+// of two floats.
+template <int V>
+__device__ __forceinline__ void norm_values(float (&h)[V], const InvRms &inv, const float (&w)[V]) {
+  if (isinf(inv.hi)) {  // (rows of subnormals without eps, NaN for zero rows)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      h[j] = __fmul_rn(__double2float_rn(__dmul_rn(static_cast<double>(h[j]), inv.full)), w[j]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; j += 2) {
+    float p0, p1, t0, t1;
+    mul2(p0, p1, h[j], h[j + 1], inv.hi);
+    t0 = __fmaf_rn(h[j], inv.hi, -p0);  // (paired sums have no free negation)
+    t1 = __fmaf_rn(h[j + 1], inv.hi, -p1);
+    fma2(t0, t1, h[j], h[j + 1], inv.lo, t0, t1);
+    add2(p0, p1, p0, p1, t0, t1);
+    mul2(h[j], h[j + 1], p0, p1, w[j], w[j + 1]);
+  }
+}
+
+// Scale of an int8 row from the maximum of |y| (quant_int8.cpp:82-84, where
+// both quotients are taken in double and rounded to f32: 127 m and s m, m the
+// middle of two floats, are never within 2^-49 of a float a or of 1, so the
+// f32 quotients are the same).
+struct RowScale {
+  float scale, inv_f;
+};
+__device__ __forceinline__ RowScale row_scale(float amax) {
+  RowScale r;
+  r.scale = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
+  r.inv_f = __fdiv_rn(1.0f, r.scale);
+  return r;
+}
+
+// A value reduced over the WPR warps of a row group, known to all of them:
+// the warps' parts meet in `slot` behind one barrier and every warp adds
+// them up. The slots of a reduction are written again two barriers later.
+template <int WPR, class V, class Op>
+__device__ __forceinline__ V group_reduce(V v, V *slot, int group, int wig, int lane, Op op) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if constexpr (WPR == 1) {
-    return finish(v);
-  } else {
+  if constexpr (WPR > 1) {
     if (lane == 0) slot[wig] = v;
     group_sync(group, WPR * 32);
-    if (wig == 0) {
-      v = slot[lane % WPR];
+    v = slot[lane % WPR];
 #pragma unroll
-      for (int o = WPR / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-      const R r = finish(v);
-      if (lane == 0) *out = r;
-    }
-    group_sync(group, WPR * 32);
-    return *out;
+    for (int o = WPR / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   }
+  return v;
+}
+
+// (not inlined: one word in a few hundred gets here, and the division's
+// registers would be taken from the rows under way)
+__device__ __noinline__ uint32_t encode4_i8_by(float4 t, float scale) {
+  return encode4_i8_exact(t, __ddiv_rn(1.0, static_cast<double>(scale)));
 }
 
 // Codes of V consecutive values of one row starting at column c. I8: from
@@ -205,20 +221,32 @@ __device__ __forceinline__ void store_codes(const NormArgs &a, int row, int c, c
   uint32_t w[V / 4];
   if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q)
-      w[q] = encode4_i8_x2(make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]), rs.inv,
-                           rs.inv_f, isinf(rs.inv_f));
+    for (int q = 0; q < V / 4; ++q) {
+      const float4 t = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+      bool tie;
+      w[q] = encode4_i8_fast(t, rs.inv_f, tie);
+      if (tie || isinf(rs.inv_f)) w[q] = encode4_i8_by(t, rs.scale);
+    }
   } else {
-    float m = 0.0f;
+    float m = 0.0f;  // (a NaN stays: the block then takes the exact encoder)
 #pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(y[j]));
+    for (int j = 0; j < V; ++j) m = max_nan(m, fabsf(y[j]));
 #pragma unroll
-    for (int o = 1; o < 32 / V; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t sc = mx_scale_code(block_pow(m, 448.0f));
+    for (int o = 1; o < 32 / V; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    uint32_t sc = mx_scale_code(m > 448.0f ? block_pow(m, 448.0f) : 0);
+    if (__any_sync(0xffffffffu, m != m)) {
+      float top = 0.0f;  // the maximum of the others
+#pragma unroll
+      for (int j = 0; j < V; ++j) top = fmaxf(top, fabsf(y[j]));
+#pragma unroll
+      for (int o = 1; o < 32 / V; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      sc = mx_scale_code(block_pow(top, 448.0f));
+    }
     const float si = e8m0_inverse(sc);
 #pragma unroll
     for (int q = 0; q < V / 4; ++q)
-      w[q] = mx_encode4_f8<kE4M3>(make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]), si);
+      w[q] = mx_encode4_f8<kE4M3>(make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]),
+                                  si, m != m);
     if (live && c % 32 == 0)
       static_cast<uint8_t *>(a.scales)[static_cast<size_t>(row) * (a.cols / 32) + c / 32] =
           static_cast<uint8_t>(sc);
@@ -232,13 +260,11 @@ __device__ __forceinline__ void store_codes(const NormArgs &a, int row, int c, c
 }
 
 template <int T, int V, int FMT, int WPR, bool RES>
-__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
+__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256, WPR > 16 ? 1 : WPR > 8 ? 2 : 3)
     norm_quant_kernel(const NormArgs a) {
   constexpr int kWarps = WPR > 8 ? WPR : 8, kGroups = kWarps / WPR, kNv = kPerThread / V;
-  __shared__ double sum_slot[kWarps];
+  __shared__ double sum_slot[2][kWarps];
   __shared__ float max_slot[kWarps];
-  __shared__ InvRms rms_out[kGroups];
-  __shared__ RowScale scale_out[kGroups];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = warp / WPR, wig = warp % WPR;
   const int c0 = (wig * 32 + lane) * V;  // first column; the next kNv - 1 are WPR * 32 * V apart
@@ -261,20 +287,17 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
   }
   int row = blockIdx.x * kGroups + group;
   if (row < a.rows) fetch(row);
-  for (; row < a.rows; row += gridDim.x * kGroups) {
+  for (int odd = 0; row < a.rows; row += gridDim.x * kGroups, odd ^= 1) {
     float h[kNv][V];
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < kNv; ++i) {
       const int c = c0 + i * kStep;
-      xr[i].unpack(h[i]);
       if constexpr (RES) {
-        float t[V];
-        rr[i].unpack(t);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = __fadd_rn(h[i][j], t[j]);
-        if (c < a.cols) round_store<T, V>(a.h, row * a.ldh + c, h[i]);
+        xr[i].add(rr[i]);
+        if (c < a.cols) xr[i].store(a.h, row * a.ldh + c);
       }
+      xr[i].unpack(h[i]);
     }
     // the next row's loads run under this row's reductions and codes
     const int next = row + gridDim.x * kGroups;
@@ -283,10 +306,9 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
     for (int i = 0; i < kNv; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = __fma_rn(static_cast<double>(h[i][j]), h[i][j], ss);
-    const InvRms inv = group_reduce<WPR>(
-        ss, sum_slot + group * WPR, rms_out + group, group, wig, lane,
-        [](double p, double q) { return __dadd_rn(p, q); },
-        [&](double v) { return split_inverse(norm_inverse(v, a.cols, a.eps)); });
+    ss = group_reduce<WPR>(ss, sum_slot[odd] + group * WPR, group, wig, lane,
+                           [](double p, double q) { return __dadd_rn(p, q); });
+    const InvRms inv = inverse_rms(ss, a.by_cols, a.eps);
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kNv; ++i) {
@@ -294,18 +316,15 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
       if (c < a.cols) {
         float wv[V];
         load_weights<V>(a.w, c, wv);
+        norm_values<V>(h[i], inv, wv);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          h[i][j] = norm_value(h[i][j], inv, wv[j]);
-          amax = fmaxf(amax, fabsf(h[i][j]));
-        }
+        for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(h[i][j]));
       }
     }
     RowScale rs{};
     if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
-      rs = group_reduce<WPR>(amax, max_slot + group * WPR, scale_out + group, group, wig, lane,
-                             [](float p, float q) { return fmaxf(p, q); },
-                             [](float v) { return row_scale(v); });
+      rs = row_scale(group_reduce<WPR>(amax, max_slot + group * WPR, group, wig, lane,
+                                       [](float p, float q) { return fmaxf(p, q); }));
       if (wig == 0 && lane == 0) static_cast<float *>(a.scales)[row] = rs.scale;
     }
 #pragma unroll
@@ -320,37 +339,35 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256)
 // reading h again (from h_out, written by the same threads, or x).
 template <int T, int V, int FMT>
 __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a) {
-  __shared__ double sum_slot[32];
+  __shared__ double sum_slot[2][32];
   __shared__ float max_slot[32];
-  __shared__ InvRms rms_out;
-  __shared__ RowScale scale_out;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const void *src = a.r ? a.h : a.x;
   const long long lds = a.r ? a.ldh : a.ldx;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int row = blockIdx.x, odd = 0; row < a.rows; row += gridDim.x, odd ^= 1) {
     double ss = 0.0;
     for (int c = threadIdx.x * V; c < a.cols; c += 1024 * V) {
-      float h[V];
-      load_vec<T, V>(a.x, row * a.ldx + c, h);
+      Raw<T, V> x;
+      x.load(a.x, row * a.ldx + c);
       if (a.r) {
-        float t[V];
-        load_vec<T, V>(a.r, row * a.ldr + c, t);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = __fadd_rn(h[j], t[j]);
-        round_store<T, V>(a.h, row * a.ldh + c, h);
+        Raw<T, V> r;
+        r.load(a.r, row * a.ldr + c);
+        x.add(r);
+        x.store(a.h, row * a.ldh + c);
       }
+      float h[V];
+      x.unpack(h);
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = __fma_rn(static_cast<double>(h[j]), h[j], ss);
     }
-    const InvRms inv = group_reduce<32>(
-        ss, sum_slot, &rms_out, 0, warp, lane, [](double p, double q) { return __dadd_rn(p, q); },
-        [&](double v) { return split_inverse(norm_inverse(v, a.cols, a.eps)); });
+    ss = group_reduce<32>(ss, sum_slot[odd], 0, warp, lane,
+                          [](double p, double q) { return __dadd_rn(p, q); });
+    const InvRms inv = inverse_rms(ss, a.by_cols, a.eps);
     auto values = [&](int c, float (&y)[V]) {
       float wv[V];
       load_vec<T, V>(src, row * lds + c, y);
       load_weights<V>(a.w, c, wv);
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = norm_value(y[j], inv, wv[j]);
+      norm_values<V>(y, inv, wv);
     };
     RowScale rs{};
     if constexpr (FMT == ROUGE_B200_Q_I8_ROWS) {
@@ -361,9 +378,8 @@ __global__ void __launch_bounds__(1024) norm_quant_long_kernel(const NormArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(y[j]));
       }
-      rs = group_reduce<32>(amax, max_slot, &scale_out, 0, warp, lane,
-                            [](float p, float q) { return fmaxf(p, q); },
-                            [](float v) { return row_scale(v); });
+      rs = row_scale(group_reduce<32>(amax, max_slot, 0, warp, lane,
+                                      [](float p, float q) { return fmaxf(p, q); }));
       if (threadIdx.x == 0) static_cast<float *>(a.scales)[row] = rs.scale;
     }
     // (whole warps: a block's lanes take part in its shuffles)
@@ -407,7 +423,7 @@ int launch_wpr(const NormArgs &a, cudaStream_t st) {
 // Warps per row: the fewest whose registers hold it.
 template <int T, int V, int FMT>
 int launch_vec(const NormArgs &a, cudaStream_t st) {
-  const int per_warp = 32 * kPerThread;
+  constexpr int per_warp = 32 * kPerThread;
   if (a.cols <= per_warp) return launch_wpr<T, V, FMT, 1>(a, st);
   if (a.cols <= 2 * per_warp) return launch_wpr<T, V, FMT, 2>(a, st);
   if (a.cols <= 4 * per_warp) return launch_wpr<T, V, FMT, 4>(a, st);
@@ -459,7 +475,7 @@ extern "C" int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const 
   const int s = device_ready();
   if (s != ROUGE_B200_OK) return s;
   if (rows == 0) return ROUGE_B200_OK;
-  NormArgs a{x, residual, ldx, ldr, ldh, w, eps, rows, cols, h_out, codes, scales};
+  NormArgs a{x, residual, ldx, ldr, ldh, w, eps, rows, cols, 1.0 / cols, h_out, codes, scales};
   cudaStream_t st = as_stream(stream);
   const bool wide = type != ROUGE_B200_T_F32 && cols % 8 == 0 && all(16) &&
                     (reinterpret_cast<uintptr_t>(codes) & 7u) == 0;
