@@ -128,6 +128,11 @@ struct GemmArgs {
   // rouge_b200_set_tile_mode; the others fix it for this call only (the
   // RougeGemmConfig of the drop-in float GEMMs).
   int tile_hint;
+  // Bytes by which the A box is shorter than 128 rows (M below 128, single
+  // CTAs): rows past M are not fetched -- a row the tensor map fills with
+  // zeros costs the copy engine more than a real one -- and what the stage
+  // holds there only reaches accumulator rows that are never stored.
+  int a_missing;
   // Clock probe (rouge_b200_set_clock_probe): CTA b < clk_n writes
   // %clock64 and %globaltimer at its start to clk[4b], clk[4b + 1] and at
   // its end to clk[4b + 2], clk[4b + 3]. Null: no stamps.
@@ -172,15 +177,26 @@ struct alignas(64) OutMaps {
   int n;
 };
 
-template <MmaKind KIND, int BN, bool B_MN>
+// A_ROWS below 128 (M at most that): the stages hold only those rows of A
+// and so four k-blocks each; the MMA reads 128 rows from a k-block's first,
+// the rest of them whatever lies behind (accumulator rows past M).
+template <MmaKind KIND, int BN, bool B_MN, int A_ROWS = kBM>
 struct Cfg {
   static constexpr int ESIZE = KIND == MmaKind::TF32 ? 4 : (KIND == MmaKind::F16 ? 2 : 1);
   static constexpr int BK = kBKBytes / ESIZE;       // elements of K per stage
   static constexpr int UMMA_K = 32 / ESIZE;         // elements of K per instruction
-  static constexpr int A_BYTES = kBM * kBKBytes;
+  static constexpr int A_BYTES = A_ROWS * kBKBytes;
   static constexpr int B_BYTES = BN * kBKBytes;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES > 8 ? 8 : (192 * 1024) / STAGE_BYTES;
+  // k-blocks per stage: a stage's round trip costs 0.13 us whatever it holds,
+  // next to 0.14 us for a few-row k-block (the shared memory's bandwidth:
+  // four MMAs read 24 KB, the copies write 10). M = 16, N = K = 8192, int8:
+  // 24.1 us with one, 20.3 with two, 18.6 with four, 20.2 with eight.
+  static constexpr int NKB = A_ROWS < kBM ? 4 : 1;
+  static constexpr int BLOCK_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGE_BYTES = NKB * BLOCK_BYTES;
+  static constexpr int MAX_STAGES = 8;
+  static constexpr int STAGES =
+      (192 * 1024) / STAGE_BYTES > MAX_STAGES ? MAX_STAGES : (192 * 1024) / STAGE_BYTES;
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int B_CHUNKS = (BN * ESIZE) / kBKBytes;  // 128-byte N chunks (MN-major B)
   static constexpr int B_CHUNK_BYTES = B_MN ? BK * kBKBytes : B_BYTES;
@@ -755,16 +771,17 @@ __device__ __forceinline__ void conv_kblock(const GemmArgs &args, int kb, int bk
   kx = tap * args.conv_cin + c0;
 }
 
-template <MmaKind KIND, int BN, bool B_MN, int OUT, bool CONV = false, bool EP = false>
+template <MmaKind KIND, int BN, bool B_MN, int OUT, bool CONV = false, bool EP = false,
+          int A_ROWS = kBM>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ OutMaps om, const GemmArgs args) {
-  using C = Cfg<KIND, BN, B_MN>;
+  using C = Cfg<KIND, BN, B_MN, A_ROWS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
   uint8_t *sA = smem;
-  uint8_t *sB = smem + C::STAGES * C::A_BYTES;
+  uint8_t *sB = smem + C::STAGES * C::NKB * C::A_BYTES;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES + C::EPI_BYTES);
   uint64_t *empty = full + C::STAGES;
   uint64_t *tfull = empty + C::STAGES;  // [2]
@@ -817,7 +834,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       tile_coords(t, args.num_m, args.num_n, mb, nb);
       int cw = 0, ch = 0, cn = 0;
       if constexpr (CONV) conv_box(args, mb * kBM, cw, ch, cn);
-      for (int kb = 0; kb < args.num_k; ++kb, ++it) {
+      for (int kb0 = 0; kb0 < args.num_k; kb0 += C::NKB, ++it) {
         const int s = it % C::STAGES;
         const uint32_t round = static_cast<uint32_t>(it / C::STAGES);
         if (!mbar_wait(&empty[s], (round & 1u) ^ 1u, abort)) {
@@ -825,24 +842,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
-        int kx = kb * C::BK;  // K coordinate of the B tile
-        if constexpr (CONV) {
-          int c0, kr, kc;
-          conv_kblock(args, kb, C::BK, c0, kr, kc, kx);
-          tma_load_im2col_4d(sA + s * C::A_BYTES, &tmA, &full[s], c0, cw, ch, cn,
-                             static_cast<uint16_t>(kc), static_cast<uint16_t>(kr));
-        } else {
-          tma_load_2d(sA + s * C::A_BYTES, &tmA, &full[s], kx, mb * kBM);
-        }
-        if constexpr (!B_MN) {
-          tma_load_2d(sB + s * C::B_BYTES, &tmB, &full[s], kx,
-                      nb * BN + (args.item_m ? (mb * kBM / args.item_m) * args.N : 0));
-        } else {
+        mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES - C::NKB * args.a_missing);
 #pragma unroll
-          for (int j = 0; j < C::B_CHUNKS; ++j)
-            tma_load_2d(sB + s * C::B_BYTES + j * C::B_CHUNK_BYTES, &tmB, &full[s],
-                        nb * BN + j * (kBKBytes / C::ESIZE), kb * C::BK);
+        for (int u = 0; u < C::NKB; ++u) {  // (k-blocks past K are filled with zeros)
+          const int kb = kb0 + u, blk = s * C::NKB + u;
+          int kx = kb * C::BK;  // K coordinate of the B tile
+          if constexpr (CONV) {
+            int c0, kr, kc;
+            conv_kblock(args, kb, C::BK, c0, kr, kc, kx);
+            tma_load_im2col_4d(sA + blk * C::A_BYTES, &tmA, &full[s], c0, cw, ch, cn,
+                               static_cast<uint16_t>(kc), static_cast<uint16_t>(kr));
+          } else {
+            tma_load_2d(sA + blk * C::A_BYTES, &tmA, &full[s], kx, mb * kBM);
+          }
+          if constexpr (!B_MN) {
+            tma_load_2d(sB + blk * C::B_BYTES, &tmB, &full[s], kx,
+                        nb * BN + (args.item_m ? (mb * kBM / args.item_m) * args.N : 0));
+          } else {
+#pragma unroll
+            for (int j = 0; j < C::B_CHUNKS; ++j)
+              tma_load_2d(sB + blk * C::B_BYTES + j * C::B_CHUNK_BYTES, &tmB, &full[s],
+                          nb * BN + j * (kBKBytes / C::ESIZE), kb * C::BK);
+          }
         }
       }
     }
@@ -874,7 +895,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       tc_fence_after_sync();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(slot * BN);
-      for (int kb = 0; kb < args.num_k; ++kb, ++it) {
+      for (int kb = 0; kb < args.num_k; kb += C::NKB, ++it) {
         const int s = it % C::STAGES;
         const uint32_t round = static_cast<uint32_t>(it / C::STAGES);
         if (!mbar_wait(&full[s], round & 1u, abort)) {
@@ -883,15 +904,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           break;
         }
         tc_fence_after_sync();
-        const uint32_t a0 = smem_u32(sA + s * C::A_BYTES);
-        const uint32_t b0 = smem_u32(sB + s * C::B_BYTES);
 #pragma unroll
-        for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
-          const uint64_t adesc = smem_desc_sw128(a0 + k * 32, 16, 1024);
-          const uint64_t bdesc =
-              B_MN ? smem_desc_sw128(b0 + k * C::UMMA_K * kBKBytes, C::B_CHUNK_BYTES, 1024)
-                   : smem_desc_sw128(b0 + k * 32, 16, 1024);
-          umma<KIND>(d_tmem, adesc, bdesc, idesc, (kb | k) != 0 ? 1u : 0u);
+        for (int u = 0; u < C::NKB; ++u) {
+          const uint32_t a0 = smem_u32(sA + (s * C::NKB + u) * C::A_BYTES);
+          const uint32_t b0 = smem_u32(sB + (s * C::NKB + u) * C::B_BYTES);
+#pragma unroll
+          for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
+            const uint64_t adesc = smem_desc_sw128(a0 + k * 32, 16, 1024);
+            const uint64_t bdesc =
+                B_MN ? smem_desc_sw128(b0 + k * C::UMMA_K * kBKBytes, C::B_CHUNK_BYTES, 1024)
+                     : smem_desc_sw128(b0 + k * 32, 16, 1024);
+            umma<KIND>(d_tmem, adesc, bdesc, idesc, (kb | u | k) != 0 ? 1u : 0u);
+          }
         }
         issued = true;
         tc_commit(&empty[s]);
@@ -930,7 +954,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       tc_fence_after_sync();
       epilogue_tile<KIND, OUT, 1, EP>(args, tmem_base + static_cast<uint32_t>(slot * BN), mb * kBM,
-                                  nb * BN, BN, quarter, half, sab, stage, seq, &om, lane);
+                                      nb * BN, BN, quarter, half, sab, stage, seq, &om, lane);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[slot]);
@@ -1606,7 +1630,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // make_b(box_rows, map) encodes the B operand's tensor map with boxes of
 // `box_rows` rows (K-major B) and returns a status.
 template <MmaKind KIND, int BN, bool B_MN, int OUT, bool CONV, bool PAIR, bool FQ = false,
-          bool EP = false, class MakeB>
+          bool EP = false, int A_ROWS = kBM, class MakeB>
 int launch_tiles(const CUtensorMap &ta, MakeB make_b, GemmArgs args, cudaStream_t st) {
   int s = ROUGE_B200_OK;
   if (unsigned long long *stamps = g_clock_stamps.load()) {
@@ -1662,8 +1686,8 @@ int launch_tiles(const CUtensorMap &ta, MakeB make_b, GemmArgs args, cudaStream_
   const unsigned long long bit = 1ull << (current_device() & 63);
   const int sms = current_sm_count();
   if constexpr (!PAIR) {
-    using C = Cfg<KIND, BN, B_MN>;
-    auto kern = gemm_tc_kernel<KIND, BN, B_MN, OUT, CONV, EP>;
+    using C = Cfg<KIND, BN, B_MN, A_ROWS>;
+    auto kern = gemm_tc_kernel<KIND, BN, B_MN, OUT, CONV, EP, A_ROWS>;
     // The shared-memory opt-in is a per-device function attribute.
     static std::atomic<unsigned long long> attr_done{0};
     if (!(attr_done.load() & bit)) {
@@ -1764,7 +1788,7 @@ int launch_tiles(const CUtensorMap &ta, MakeB make_b, GemmArgs args, cudaStream_
   }
 }
 
-template <MmaKind KIND, int BN, bool B_MN, int OUT, bool PAIR, bool EP = false>
+template <MmaKind KIND, int BN, bool B_MN, int OUT, bool PAIR, bool EP = false, int A_ROWS = kBM>
 int launch_gemm_impl(const void *A, long long lda, const void *B, long long ldb, GemmArgs args,
                      cudaStream_t st) {
   using C = Cfg<KIND, BN, B_MN>;
@@ -1772,8 +1796,10 @@ int launch_gemm_impl(const void *A, long long lda, const void *B, long long ldb,
                                  : C::ESIZE == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUtensorMap ta;
+  const int a_box = !PAIR && args.M < A_ROWS ? (args.M + 7) / 8 * 8 : A_ROWS;
+  args.a_missing = (A_ROWS - a_box) * kBKBytes;
   int s = make_tmap_2d(&ta, A, dt, args.K, args.M, static_cast<uint64_t>(lda) * C::ESIZE, C::BK,
-                       kBM);
+                       a_box);
   if (s != ROUGE_B200_OK) return s;
   auto make_b = [&](int box_rows, CUtensorMap *tb) {
     if (!B_MN)  // K-major: boxes of box_rows rows of B (every item's rows when batched)
@@ -1783,17 +1809,17 @@ int launch_gemm_impl(const void *A, long long lda, const void *B, long long ldb,
     return make_tmap_2d(tb, B, dt, args.N, args.K, static_cast<uint64_t>(ldb) * C::ESIZE,
                         kBKBytes / C::ESIZE, C::BK);
   };
-  return launch_tiles<KIND, BN, B_MN, OUT, false, PAIR, false, EP>(ta, make_b, args, st);
+  return launch_tiles<KIND, BN, B_MN, OUT, false, PAIR, false, EP, A_ROWS>(ta, make_b, args, st);
 }
 
-template <MmaKind KIND, int BN, bool B_MN, bool PAIR, bool EP>
+template <MmaKind KIND, int BN, bool B_MN, bool PAIR, bool EP, int A_ROWS = kBM>
 int launch_out(const void *A, long long lda, const void *B, long long ldb, GemmArgs args,
                int out_type, cudaStream_t st) {
   switch (out_type) {
     case ROUGE_B200_OUT_F32:
-      return launch_gemm_impl<KIND, BN, B_MN, ROUGE_B200_OUT_F32, PAIR, EP>(A, lda, B, ldb, args, st);
+      return launch_gemm_impl<KIND, BN, B_MN, ROUGE_B200_OUT_F32, PAIR, EP, A_ROWS>(A, lda, B, ldb, args, st);
     case ROUGE_B200_OUT_BF16:
-      return launch_gemm_impl<KIND, BN, B_MN, ROUGE_B200_OUT_BF16, PAIR, EP>(A, lda, B, ldb, args, st);
+      return launch_gemm_impl<KIND, BN, B_MN, ROUGE_B200_OUT_BF16, PAIR, EP, A_ROWS>(A, lda, B, ldb, args, st);
     default:
       if constexpr (KIND == MmaKind::I8 && !EP)
         return launch_gemm_impl<KIND, BN, B_MN, ROUGE_B200_OUT_I32, PAIR>(A, lda, B, ldb, args,
@@ -1854,6 +1880,12 @@ int launch_kind(const void *A, long long lda, const void *B, long long ldb, int 
     const bool n32 = 4 * args.num_tiles <= current_sm_count();
     args.num_n = (args.N + (n32 ? 31 : 63)) / (n32 ? 32 : 64);
     args.num_tiles = args.num_m * args.num_n;
+    // At most 32 rows (a decoding step): the weights' bytes are the work, and
+    // the per-stage costs are spread over four k-blocks (Cfg::NKB).
+    if constexpr (EP)
+      if (args.M <= 32)
+        return n32 ? launch_out<KIND, 32, false, false, EP, 32>(A, lda, B, ldb, args, out_type, st)
+                   : launch_out<KIND, 64, false, false, EP, 32>(A, lda, B, ldb, args, out_type, st);
     return n32 ? launch_out<KIND, 32, false, false, EP>(A, lda, B, ldb, args, out_type, st)
                : launch_out<KIND, 64, false, false, EP>(A, lda, B, ldb, args, out_type, st);
   }
