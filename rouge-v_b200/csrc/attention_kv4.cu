@@ -32,35 +32,14 @@
 #include <cmath>
 #include <cstdint>
 
-#include "kv4.cuh"
+#include "attention_kv4.cuh"
 #include "ptx.cuh"
-#include "x86fp.cuh"
 
 namespace rb200 {
 namespace {
 
 constexpr int kTile = 32;   // keys per tile
 constexpr int kMinTilesLog2 = 1;  // two tiles per warp before another warp joins
-
-struct AttnArgs {
-  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
-  const float *gs_k, *gs_v;
-  int pages, page, Hkv, Dh;
-  const void *Q;
-  void *O;
-  int B, Hq, group;
-  const int *cu_q;
-  int max_q;
-  const int *kv_len;
-  const int *page_table;
-  int max_pages;
-  float scale;
-  int causal, window;
-  int warps;      // warps of the grid
-  float *part;    // [2 * warps][rows * (Dh + 4)]: weighted sums, then maximum and sum per row
-  int4 *desc;     // [2 * warps]: sequence, head, row tile, valid
-  int *err;
-};
 
 struct SeqInfo {
   int nq, len, q0;     // queries (at most max_q), keys, first query
@@ -93,9 +72,6 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
   return a / b;
 }
 
-// 2^e for -126 <= e <= 127.
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -110,12 +86,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Key (of 16) in row r of the score products' A fragments. Lane t's rows 2t,
 // 2t + 1, 2t + 8 and 2t + 9 of the weights hold the keys t, 4 + (t ^ 1), and
 // 8 more: the four value rows a load reads then lie in two bank halves, and
@@ -123,46 +93,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ int key_of_row(int r) {
   const int q = (r & 7) >> 1;
   return (r & 8) + ((r & 1) ? 4 + (q ^ 1) : q);
-}
-
-// 16 consecutive query values (16-byte aligned).
-template <int T>
-__device__ __forceinline__ void load_q16(const void *q, long long at, float *v) {
-  if constexpr (T == ROUGE_B200_T_F32) {
-    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 t = p[i];
-      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
-    }
-  } else {
-    const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + at);
-    const uint4 t0 = p[0], t1 = p[1];
-    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (T == ROUGE_B200_T_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-      }
-    }
-  }
-}
-
-// Four consecutive output values (aligned to four).
-template <int T>
-__device__ __forceinline__ void store_o4(void *o, long long at, float x, float y, float z, float w) {
-  if constexpr (T == ROUGE_B200_T_F32)
-    *reinterpret_cast<float4 *>(static_cast<float *>(o) + at) = make_float4(x, y, z, w);
-  else if constexpr (T == ROUGE_B200_T_F16)
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
-        make_uint2(f16x2_rn(x, y), f16x2_rn(z, w));
-  else
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
-        make_uint2(bf16x2_rn(x, y), bf16x2_rn(z, w));
 }
 
 // Warps per block and blocks per SM: 16 warps an SM where a warp's O^T
@@ -376,13 +306,9 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         for (int k = 0; k < DT / 4; ++k) m = fmaxf(m, fabsf(v[k]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        // exponent of the row maximum (0 for an empty or unbounded row)
-        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
-        if (e == 128) e = 0;             // (infinity or NaN)
-        e = e < -100 ? -100 : e;         // (tiny rows stay tiny)
-        const float down = pow2(-(e / 2)), down2 = pow2(-(e - e / 2));
+        const RowExponent re = row_exponent(m);
 #pragma unroll
-        for (int k = 0; k < DT / 4; ++k) v[k] = v[k] * down * down2;
+        for (int k = 0; k < DT / 4; ++k) v[k] = v[k] * re.down * re.down2;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -395,8 +321,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
               qf[S::NR + j][s][p] = f16x2_rn(x0 - b2.x, x1 - b2.y);
             }
           }
-        // (kept positive: a masked score is -inf before it is scaled)
-        const float mine = fmaxf(a.scale * 1.44269504f * gk * pow2(e / 2) * pow2(e - e / 2), 1e-37f);
+        const float mine = row_factor(re, a.scale, gk);
         mult[j][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
         mult[j][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
       }
@@ -913,6 +838,7 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   a.err = device_error_word();
   if (!a.err) return set_status(ROUGE_B200_ENOMEM);
   cudaStream_t st = as_stream(stream);
+  if (kv4_tiles_apply(a, type)) return launch_attention_kv4_tiles(a, type, st);
   if (a.Dh <= 64) return launch_dt<64>(a, type, rt_rows, st);
   if (a.Dh <= 128) return launch_dt<128>(a, type, rt_rows, st);
   return launch_dt<256>(a, type, rt_rows, st);

@@ -1,0 +1,113 @@
+// What the kernels of the attention over the 4-bit cache share: their
+// arguments, query loads, output stores.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "kv4.cuh"
+#include "x86fp.cuh"
+
+namespace rb200 {
+
+struct AttnArgs {
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const float *gs_k, *gs_v;
+  int pages, page, Hkv, Dh;
+  const void *Q;
+  void *O;
+  int B, Hq, group;
+  const int *cu_q;
+  int max_q;
+  const int *kv_len;
+  const int *page_table;
+  int max_pages;
+  float scale;
+  int causal, window;
+  int warps;      // warps of the grid
+  float *part;    // [2 * warps][rows * (Dh + 4)]: weighted sums, then maximum and sum per row
+  int4 *desc;     // [2 * warps]: sequence, head, row tile, valid
+  int *err;
+};
+
+// Long prompt chunks on the tensor cores (attention_kv4_tiles.cu): whether
+// that kernel takes the call, and its launch.
+bool kv4_tiles_apply(const AttnArgs &a, int type);
+int launch_attention_kv4_tiles(const AttnArgs &a, int type, cudaStream_t st);
+
+namespace {
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// The power-of-two exponent of a row of queries whose largest magnitude is m,
+// and factors that take it out: the row is scaled to [1, 2) before it is
+// rounded to f16, the scores by 2^e afterwards.
+struct RowExponent {
+  int e;
+  float down, down2;
+};
+__device__ __forceinline__ RowExponent row_exponent(float m) {
+  RowExponent r;
+  r.e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+  if (r.e == 128) r.e = 0;          // (infinity or NaN)
+  r.e = r.e < -100 ? -100 : r.e;    // (tiny rows stay tiny)
+  r.down = pow2(-(r.e / 2));
+  r.down2 = pow2(-(r.e - r.e / 2));
+  return r;
+}
+// Factor of a row's raw scores to base-2 logits; kept positive, since a
+// masked score is -inf before it is scaled.
+__device__ __forceinline__ float row_factor(const RowExponent &r, float scale, float gk) {
+  return fmaxf(scale * 1.44269504f * gk * pow2(r.e / 2) * pow2(r.e - r.e / 2), 1e-37f);
+}
+
+// 16 consecutive query values (16-byte aligned).
+template <int T>
+__device__ __forceinline__ void load_q16(const void *q, long long at, float *v) {
+  if constexpr (T == ROUGE_B200_T_F32) {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 t = p[i];
+      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+    }
+  } else {
+    const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + at);
+    const uint4 t0 = p[0], t1 = p[1];
+    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (T == ROUGE_B200_T_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+// Four consecutive output values (aligned to four).
+template <int T>
+__device__ __forceinline__ void store_o4(void *o, long long at, float x, float y, float z, float w) {
+  if constexpr (T == ROUGE_B200_T_F32)
+    *reinterpret_cast<float4 *>(static_cast<float *>(o) + at) = make_float4(x, y, z, w);
+  else if constexpr (T == ROUGE_B200_T_F16)
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
+        make_uint2(f16x2_rn(x, y), f16x2_rn(z, w));
+  else
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + at) =
+        make_uint2(bf16x2_rn(x, y), bf16x2_rn(z, w));
+}
+
+}  // namespace
+}  // namespace rb200

@@ -1,0 +1,437 @@
+// Attention over the paged 4-bit cache for long prompt chunks: 256 query
+// rows (two tiles of 128; the group's heads times the queries) per block on
+// the tcgen05 tensor cores, 128 keys at a time.
+//
+//   warps 0-3, 4-7  softmax of row tile 0 and 1: one thread per row. Scores
+//                   from TMEM, running maximum and sum, weights as f16 back
+//                   to TMEM (over the scores), O rescaled when the maximum
+//                   has grown by more than 2^8
+//   warps 8-11      one thread per key: codes from the pages to f16 K and V
+//                   rows in shared memory (128-byte swizzle), one block ahead
+//   warp 12         issues S = Q K^T (operands in shared memory) and O += P V
+//                   (P in TMEM, V as it lies: keys x d, the N-major operand)
+//
+// While one tile's softmax runs, the tensor cores work on the other. The
+// scores' columns hold the weights afterwards, so a tile's next S is issued
+// when its O += P V has completed; a tile's S in hand thus also means that
+// its O is up to date and may be rescaled.
+//
+// What bounds it: per 128 x 128 block of one tile at Dh 128 the two products
+// take 1024 cycles at the measured matrix rate, the 16384 exponentials as
+// many on 16 lanes a cycle. code * scale is exact in f16, as are 16-bit
+// queries scaled by a power of two per row; weights are rounded to f16.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+
+#include "attention_kv4.cuh"
+#include "ptx.cuh"
+
+namespace rb200 {
+namespace {
+
+constexpr int kThreads = 13 * 32;
+constexpr int kKeys = 128;           // per block of keys
+constexpr int kRows = 256;           // per CTA
+constexpr uint32_t kChunk = 16384;   // 128 rows x 128 bytes (64 f16)
+constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
+constexpr float kTop = 7.0f;         // weights are held times 2^7: at most 2^15
+
+template <int DH>
+struct TileCfg {
+  static constexpr int CH = DH / 64;                       // 64-value chunks of a row
+  static constexpr uint32_t TILE = CH * kChunk;            // one tile of Q, K or V
+  static constexpr uint32_t SMEM = 1024 + 6 * TILE + 256;  // Q x 2, K x 2, V x 2, barriers
+  static constexpr uint32_t O_COL = 256;                   // TMEM: S0 0, S1 128, O0 256, O1
+  static constexpr uint32_t COLS = 512;
+};
+
+// 8 codes (one 32-bit word) times a scale pair as one 16-byte unit of f16.
+__device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t scale2) {
+  uint32_t h[4];
+  e2m1x8_f16x2(w, h);
+  return make_uint4(mul_f16x2(h[0], scale2), mul_f16x2(h[1], scale2), mul_f16x2(h[2], scale2),
+                    mul_f16x2(h[3], scale2));
+}
+
+// Byte offset of 16-byte unit u (8 values) of row r in a swizzled tile.
+__device__ __forceinline__ uint32_t unit_at(int r, int u) {
+  return (u >> 3) * kChunk + r * 128 + (((u & 7) ^ (r & 7)) << 4);
+}
+
+template <int DH>
+struct KeyRow {  // one key's codes and scales of K or V
+  uint4 c[DH / 32];
+  uint32_t s[DH / 64];  // four scales each
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) c[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < DH / 64; ++i) s[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, size_t row) {
+    const uint4 *p = reinterpret_cast<const uint4 *>(codes + row * (DH / 2));
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) c[i] = __ldg(p + i);
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(scales + row * (DH / 16));
+#pragma unroll
+    for (int i = 0; i < DH / 64; ++i) s[i] = __ldg(q + i);
+  }
+  __device__ __forceinline__ void write(uint32_t tile, int r) const {
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b) {
+      const uint32_t h = e4m3x2_f16x2((s[b / 4] >> (8 * (b & 3))) & 0xFFu);
+      const uint32_t s2 = __byte_perm(h, h, 0x1010);
+      const uint4 v = c[b / 2];
+      const uint32_t w0 = (b & 1) ? v.z : v.x, w1 = (b & 1) ? v.w : v.y;
+      const uint4 x = decode8(w0, s2), y = decode8(w1, s2);
+      st_shared_v4(tile + unit_at(r, 2 * b), x.x, x.y, x.z, x.w);
+      st_shared_v4(tile + unit_at(r, 2 * b + 1), y.x, y.y, y.z, y.w);
+    }
+  }
+};
+
+template <int DH, int T>
+__global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const AttnArgs a, int pairs) {
+  using C = TileCfg<DH>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~static_cast<uintptr_t>(1023));
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * C::TILE, v_s = k_s + 2 * C::TILE;
+  uint64_t *bar = reinterpret_cast<uint64_t *>(smem + 6 * C::TILE);
+  uint64_t *q_full = bar, *k_full = bar + 1, *v_full = bar + 3, *k_empty = bar + 5, *v_empty = bar + 7,
+           *s_full = bar + 9, *p_full = bar + 11, *pv_done = bar + 13, *drain = bar + 15;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 16);
+  volatile int *abort = reinterpret_cast<volatile int *>(bar + 17);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // unit: the last row tiles, which see the most keys, first
+  const int per_seq = pairs * a.Hkv;
+  const int b = blockIdx.x / per_seq, rem = blockIdx.x - b * per_seq;
+  const int pair = pairs - 1 - rem / a.Hkv, hk = rem % a.Hkv;
+  const int q0 = a.cu_q ? __ldg(a.cu_q + b) : b;
+  const int n_all = a.cu_q ? __ldg(a.cu_q + b + 1) - q0 : 1;
+  const int nq = max(0, min(n_all, a.max_q)), nrows = nq * a.group;
+  const int r0 = pair * kRows;
+  if (r0 >= nrows) return;
+  const int len = max(0, __ldg(a.kv_len + b)), p0 = len - n_all;
+  const int r1 = min(r0 + kRows, nrows) - 1;
+  const int hi_max = a.causal ? max(0, min(len, p0 + r1 / a.group + 1)) : len;
+  const int lo_min = a.window > 0 ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
+  const int first = lo_min / kKeys * kKeys;
+  const int blocks = hi_max > first ? (hi_max - first + kKeys - 1) / kKeys : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, kRows);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 128);
+      mbar_init(&v_full[i], 128);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&]() {
+    *abort = 1;
+    atomicCAS(a.err, 0, ROUGE_B200_ETIMEOUT);
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    const int w = warp >> 2, tr = threadIdx.x & 127;  // tile, row in it
+    const int r = r0 + w * 128 + tr;
+    const bool live = r < nrows;
+    const int qi = q0 + (live ? r / a.group : 0), head = hk * a.group + (live ? r % a.group : 0);
+    const long long at = (static_cast<long long>(qi) * a.Hq + head) * DH;
+    const int pos = p0 + r / a.group;
+    const int col_hi = live ? (a.causal ? min(len, pos + 1) : len) : 0x7fffffff;
+    const int col_lo = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    float mult;
+    {  // the query row, scaled to [1, 2), as f16 into the tile
+      float m = 0.0f, v[16];
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k) {
+          load_q16<T>(a.Q, at + 16 * k, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+        }
+      }
+      const RowExponent re = row_exponent(m);
+      mult = row_factor(re, a.scale, a.gs_k ? __ldg(a.gs_k + hk) : 1.0f);
+#pragma unroll
+      for (int k = 0; k < DH / 16; ++k) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        if (live) load_q16<T>(a.Q, at + 16 * k, v);
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          h[i] = f16x2_rn(v[2 * i] * re.down * re.down2, v[2 * i + 1] * re.down * re.down2);
+        st_shared_v4(q_s + w * C::TILE + unit_at(tr, 2 * k), h[0], h[1], h[2], h[3]);
+        st_shared_v4(q_s + w * C::TILE + unit_at(tr, 2 * k + 1), h[4], h[5], h[6], h[7]);
+      }
+      fence_async_smem();
+      mbar_arrive(q_full);
+    }
+    const uint32_t row_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + w * 128 + row_lane, o_t = tmem + C::O_COL + w * DH + row_lane;
+    float top = -INFINITY, sum = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < blocks; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[w], j & 1, abort));
+      if (!ok) {
+        if (lane == 0) fail();
+        break;
+      }
+      tc_fence_after_sync();
+      const int key0 = first + j * kKeys;
+      const bool whole = __all_sync(0xffffffffu, key0 >= col_lo && key0 + kKeys <= col_hi);
+      uint32_t x[2][32];
+      float m = -INFINITY;
+      tmem_ld_32x32b_x32(s_t, x[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait_regs(x[c & 1]);
+        if (c < 3) tmem_ld_32x32b_x32(s_t + 32 * (c + 1), x[(c + 1) & 1]);
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            m = max3(m, __uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int key = key0 + 32 * c + i;
+            if (key >= col_lo && key < col_hi) m = fmaxf(m, __uint_as_float(x[c & 1][i]));
+          }
+        }
+      }
+      const float logit = m * mult;
+      const bool grow = logit > top + kGrow;  // (the first keys of a row always)
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? ex2(top - logit) : 1.0f;
+        if (grow) top = logit;
+        sum *= f;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DH / 16; ++c) {
+            uint32_t y[16];
+            tmem_ld_32x32b_x16(o_t + 16 * c, y);
+            tmem_ld_wait_regs16(y);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_st_32x32b_x16(o_t + 16 * c, y);
+          }
+        }
+      }
+      const float off = top == -INFINITY ? 0.0f : kTop - top;
+      tmem_ld_32x32b_x32(s_t, x[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait_regs(x[c & 1]);
+        if (c < 3) tmem_ld_32x32b_x32(s_t + 32 * (c + 1), x[(c + 1) & 1]);
+        uint32_t h[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float u0 = __uint_as_float(x[c & 1][i]), u1 = __uint_as_float(x[c & 1][i + 1]);
+          if (!whole) {
+            const int key = key0 + 32 * c + i;
+            if (key < col_lo || key >= col_hi) u0 = -INFINITY;
+            if (key + 1 < col_lo || key + 1 >= col_hi) u1 = -INFINITY;
+          }
+          u0 = ex2(__fmaf_rn(u0, mult, off));
+          u1 = ex2(__fmaf_rn(u1, mult, off));
+          sum += u0 + u1;
+          h[i / 2] = f16x2_rn(u0, u1);
+        }
+        // (weights of keys 32c .. lie over scores that this lane has read:
+        // columns 16c .. 16c + 15; chunk c + 1, still on its way, is behind)
+        tmem_st_32x32b_x16(s_t + 16 * c, h);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(&p_full[w]);
+    }
+    if (ok && blocks > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[w], (blocks - 1) & 1, abort));
+      if (!ok && lane == 0) fail();
+      tc_fence_after_sync();
+    }
+    if (ok) {
+      const float gv = a.gs_v ? __ldg(a.gs_v + hk) : 1.0f;
+      const float f = sum > 0.0f || sum != sum ? gv / sum : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t y[32];
+        if (blocks > 0) {
+          tmem_ld_32x32b_x32(o_t + 32 * c, y);
+          tmem_ld_wait_regs(y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = 0u;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // (a row without keys: O may hold anything times zero)
+            v[k] = f == 0.0f ? 0.0f : __uint_as_float(y[i + k]) * f;
+          store_o4<T>(a.O, at + 32 * c + i, v[0], v[1], v[2], v[3]);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ K and V rows
+    const int kr = threadIdx.x - 256;
+    const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+    KeyRow<DH> k, v;
+    auto fetch = [&](int j) {
+      k.zero();
+      v.zero();
+      const int key = first + j * kKeys + kr;
+      if (j >= blocks || key >= hi_max || key < lo_min) return;  // (a key of no row: zeros)
+      const int pi = key / a.page;
+      const int id = pi < a.max_pages ? __ldg(table + pi) : -1;
+      if (id < 0 || id >= a.pages) {
+        atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
+        return;
+      }
+      const size_t row = (static_cast<size_t>(id) * a.Hkv + hk) * a.page + (key - pi * a.page);
+      k.load(a.k_codes, a.k_scales, row);
+      v.load(a.v_codes, a.v_scales, row);
+    };
+    fetch(0);
+    for (int j = 0; j < blocks; ++j) {
+      const int s = j & 1;
+      const uint32_t free = ((j >> 1) & 1) ^ 1u;
+      if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[s], free, abort))) {
+        if (lane == 0) fail();
+        break;
+      }
+      k.write(k_s + s * C::TILE, kr);
+      fence_async_smem();
+      mbar_arrive(&k_full[s]);
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[s], free, abort))) {
+        if (lane == 0) fail();
+        break;
+      }
+      v.write(v_s + s * C::TILE, kr);
+      fence_async_smem();
+      mbar_arrive(&v_full[s]);
+      fetch(j + 1);
+    }
+  } else if (lane == 0 && blocks > 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t id_s = make_idesc(1u, 0u, 0u, 0u, 0u, 128, kKeys);
+    const uint32_t id_o = make_idesc(1u, 0u, 0u, 0u, 1u, 128, DH);
+    bool issued = false;
+    auto scores = [&](int w, int s) {  // S_w = Q_w K_s^T
+#pragma unroll
+      for (int k = 0; k < DH / 16; ++k) {
+        const uint32_t step = (k >> 2) * kChunk + (k & 3) * 32;
+        umma<MmaKind::F16>(tmem + w * 128, smem_desc_sw128(q_s + w * C::TILE + step, 16, 1024),
+                           smem_desc_sw128(k_s + s * C::TILE + step, 16, 1024), id_s, k != 0);
+      }
+      tc_commit(&s_full[w]);
+      issued = true;
+    };
+    auto run = [&]() {
+      if (!mbar_wait(q_full, 0, abort) || !mbar_wait(&k_full[0], 0, abort)) return false;
+      tc_fence_after_sync();
+      scores(0, 0);
+      scores(1, 0);
+      tc_commit(&k_empty[0]);
+      for (int j = 0; j < blocks; ++j) {
+        const int s = j & 1, sn = s ^ 1;
+        for (int w = 0; w < 2; ++w) {
+          if (!mbar_wait(&p_full[w], j & 1, abort)) return false;
+          if (w == 0 && !mbar_wait(&v_full[s], (j >> 1) & 1, abort)) return false;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_f16_ta(tmem + C::O_COL + w * DH, tmem + w * 128 + 8 * k,
+                        smem_desc_sw128(v_s + s * C::TILE + k * 16 * 128, kChunk, 1024), id_o,
+                        (j | k) != 0);
+          tc_commit(&pv_done[w]);
+          if (w == 1) tc_commit(&v_empty[s]);
+          if (j + 1 < blocks) {
+            if (w == 0 && !mbar_wait(&k_full[sn], ((j + 1) >> 1) & 1, abort)) return false;
+            if (!mbar_wait(&pv_done[w], j & 1, abort)) return false;
+            tc_fence_after_sync();
+            scores(w, sn);
+            if (w == 1) tc_commit(&k_empty[sn]);
+          }
+        }
+      }
+      return true;
+    };
+    if (!run()) {
+      fail();
+      if (issued) {  // the MMAs already issued complete before TMEM is released
+        const volatile int never = 0;
+        tc_commit(drain);
+        mbar_wait(drain, 0, &never);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+template <int DH, int T>
+int launch_tiles(const AttnArgs &a, int pairs, cudaStream_t st) {
+  using C = TileCfg<DH>;
+  static_assert(C::SMEM <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
+  auto kern = attention_kv4_tiles_kernel<DH, T>;
+  static std::atomic<unsigned long long> attr_done{0};
+  const unsigned long long bit = 1ull << (current_device() & 63);
+  if (!(attr_done.load() & bit)) {
+    const int s = cuda_status(
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    if (s != ROUGE_B200_OK) return s;
+    attr_done.fetch_or(bit);
+  }
+  kern<<<static_cast<unsigned>(pairs) * a.Hkv * a.B, kThreads, C::SMEM, st>>>(a, pairs);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+bool kv4_tiles_apply(const AttnArgs &a, int type) {
+  const double rows = static_cast<double>(a.max_q) * a.group;
+  const double ctas = std::ceil(rows / kRows) * a.Hkv * a.B;
+  return type != ROUGE_B200_T_F32 && (a.Dh == 64 || a.Dh == 128) && rows >= 64 &&
+         rows * a.Hkv * a.B >= 24.0 * kRows && ctas < 2147483648.0;
+}
+
+int launch_attention_kv4_tiles(const AttnArgs &a, int type, cudaStream_t st) {
+  const int pairs = (a.max_q * a.group + kRows - 1) / kRows;
+  if (a.Dh == 64)
+    return type == ROUGE_B200_T_F16 ? launch_tiles<64, ROUGE_B200_T_F16>(a, pairs, st)
+                                    : launch_tiles<64, ROUGE_B200_T_BF16>(a, pairs, st);
+  return type == ROUGE_B200_T_F16 ? launch_tiles<128, ROUGE_B200_T_F16>(a, pairs, st)
+                                  : launch_tiles<128, ROUGE_B200_T_BF16>(a, pairs, st);
+}
+
+}  // namespace rb200

@@ -10,10 +10,11 @@ call it ds --, each weight is off by a factor within 2 ds, the exponential's
 split it: 2^-21); the weighted sums add one 2^-23 per 16 keys of a warp's run
 and per joined part. So |O - exact| <= (2 ds + w + n 2^-23) sum_t p_t |v_t|,
 plus half a step of the output's type. Below the normal f16 range a weight is off
-by half a subnormal step instead: the kernel holds 2^15 exp(s - max) in f16, whose
-subnormal step is 2^-24, so a weight relative to the largest one is off by at
-most 2^-25 / 2^15 = 2^-40, and O (divided by a sum of at least 1) by
-2^-40 sum_t |v_t|. (It shows where the heavy keys hold zeros in a column.) The
+by half a subnormal step instead: the kernels hold exp(s - max) in f16 times 2^15
+(long prompt chunks: the largest one between 2^7 and 2^15), whose subnormal step
+is 2^-24, so a weight relative to the largest one is off by at most 2^-25 / 2^15 =
+2^-40 (chunks: 2^-32), and O (divided by a sum of at least 1) by as much of
+sum_t |v_t|. (It shows where the heavy keys hold zeros in a column.) The
 output's half step is eps / 2 of the value, or half the subnormal step, which is
 smallest_normal * eps / 2, for values that f16 holds as subnormals."""
 import math
@@ -78,7 +79,7 @@ def _cache(rb, pages, Hkv, page, Dh, seed, gs=True):
     return rb.KV4Cache(by(Dh // 2), sc(), by(Dh // 2), sc(), gg(), gg())
 
 
-def _reference(cache, q, lens, table, nqs, causal, window, scale):
+def _reference(cache, q, lens, table, nqs, causal, window, scale, tiny_step=2.0 ** -40):
     """O and the tolerance's parts in 64 bits, sequence by sequence."""
     import torch
     kc, ks, vc, vs, gk, gv = cache.tensors
@@ -103,7 +104,7 @@ def _reference(cache, q, lens, table, nqs, causal, window, scale):
                 w = torch.softmax(z, 1)
                 out[at] = torch.einsum("ht,thd->hd", w, v)
                 spread[at] = torch.einsum("ht,thd->hd", w, v.abs())
-                tiny[at] = 2.0 ** -40 * v.abs().sum(0)
+                tiny[at] = tiny_step * v.abs().sum(0)
                 ds[at] = (za.amax(1) * (cache.Dh / 16 + 6) * 2.0 ** -23)[:, None]
             at += 1
     return out, spread, ds, tiny
@@ -132,12 +133,13 @@ def _attend(rb, cache, t, lens, nqs, Hq, causal=1, window=0, scale=0.0, seed=0, 
     return q, O, table, lens_d, cu
 
 
-def _check(rb, cache, t, lens, nqs, Hq, causal=1, window=0, scale=0.0, **kw):
+def _check(rb, cache, t, lens, nqs, Hq, causal=1, window=0, scale=0.0, tiny_step=2.0 ** -40, **kw):
     import torch
     q, O, table, _, _ = _attend(rb, cache, t, lens, nqs, Hq, causal, window, scale, **kw)
     rb.sync_status()
     T = sum(nqs)
-    want, spread, ds, tiny = _reference(cache, q, lens, table, nqs, causal, window, scale or 1 / math.sqrt(cache.Dh))
+    want, spread, ds, tiny = _reference(cache, q, lens, table, nqs, causal, window, scale or 1 / math.sqrt(cache.Dh),
+                                        tiny_step)
     w = 2.0 ** -21 + (2.0 ** -21 if t == "f32" else 2.0 ** -11)
     n = max(max(lens), 16) / 16 + 64
     tol = (2 * ds + w + n * 2.0 ** -23) * spread + tiny
@@ -272,6 +274,69 @@ def test_prompt_chunks(rb, cuda, nq, n, t, Hq, Hkv, Dh):
     cache = _cache(rb, 2 * (-(-n // 32)) + 2, Hkv, 32, Dh, nq, gs=False)
     _check(rb, cache, t, [n, n - 1 if n > nq else n], [nq, nq], Hq)
     _check(rb, cache, t, [n], [nq], Hq, window=20)
+
+
+@pytest.mark.parametrize("causal,window", [(1, 0), (0, 0), (1, 150), (0, 1)])
+@pytest.mark.parametrize("t,Hq,Hkv,Dh,page", [("bf16", 16, 4, 128, 64), ("f16", 9, 3, 64, 16), ("bf16", 24, 8, 128, 48),
+                                              ("bf16", 64, 1, 64, 32)])
+def test_long_prompt_chunks(rb, cuda, t, Hq, Hkv, Dh, page, causal, window):
+    """Enough rows for the kernel of 256-row tiles: ragged numbers of queries, more queries than keys, none, one."""
+    lens, nqs = [700, 130, 64, 290, 5], [301, 130, 200, 0, 1]
+    nqs = [n * 2 for n in nqs] if Hq == 9 else nqs
+    cache = _cache(rb, sum(-(-n // page) for n in lens) + 1, Hkv, page, Dh, Hq, gs=window == 0)
+    _check(rb, cache, t, lens, nqs, Hq, causal, window, extra=2, tiny_step=2.0 ** -32)
+
+
+def test_long_chunks_masked_nan_bad_pages_and_same_bits(rb, cuda):
+    import torch
+    page, lens, nqs, window = 16, [400, 260], [256, 256], 70
+    cache = _cache(rb, 60, 2, page, 128, 4)
+    ids = torch.randperm(60).tolist()
+    table = torch.full((2, 25), 1 << 30, dtype=torch.int32, device="cuda")
+    seen = torch.zeros(60, page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            table[b, i] = ids.pop()
+        for k in range(max(0, n - nqs[b] - window + 1), n):
+            seen[table[b, k // page].item(), k % page] = True
+    args = ("bf16", lens, nqs, 32)
+    clean = _check(rb, cache, *args, window=window, table=table, tiny_step=2.0 ** -32)
+    for s in (cache.tensors[1], cache.tensors[3]):
+        s.transpose(1, 2)[~seen.cuda()] = 0x7F
+    _, O, *_ = _attend(rb, cache, *args, window=window, table=table)
+    rb.sync_status()
+    assert torch.equal(O, clean)
+    table[0, 0] = -1  # wholly before the first query's window
+    _, O, *_ = _attend(rb, cache, *args, window=window, table=table)
+    rb.sync_status()
+    assert torch.equal(O, clean)
+    table[0, 20] = 60  # a page that a query needs
+    _, O, *_ = _attend(rb, cache, *args, window=window, table=table)
+    with pytest.raises(rb.RougeB200Error) as e:
+        rb.sync_status()
+    assert e.value.status == rb.EINVAL
+    assert torch.equal(O[nqs[0]:], clean[nqs[0]:]) and O.isfinite().all()
+
+
+def test_long_chunks_growing_scores(rb, cuda):
+    """Keys whose scores grow along the sequence: the running maximum moves in every block of keys."""
+    import torch
+    cache = rb.KV4Cache.empty(20, 4, 64, 128)
+    g = torch.Generator("cuda").manual_seed(2)
+    n, nq = 1280, 400
+    x = torch.randn(1, 4, 128, generator=g, device="cuda")
+    K = x * torch.linspace(0.1, 4, n, device="cuda")[:, None, None] + 0.3 * torch.randn(n, 4, 128, generator=g, device="cuda")
+    V = torch.randn(n, 4, 128, generator=g, device="cuda")
+    rb.kv4_write(cache, K, V, torch.arange(n, dtype=torch.int32, device="cuda"))
+    table = torch.arange(20, dtype=torch.int32, device="cuda")[None].contiguous()
+    q = (1.5 * x.repeat_interleave(4, 1) + 0.3 * torch.randn(nq, 16, 128, generator=g, device="cuda")).bfloat16()
+    lens, cu = torch.tensor([n], dtype=torch.int32, device="cuda"), torch.tensor([0, nq], dtype=torch.int32, device="cuda")
+    O = rb.attention_kv4(q, cache, lens, table, cu_q=cu, max_q=nq)
+    rb.sync_status()
+    want, spread, ds, tiny = _reference(cache, q, [n], table, [nq], 1, 0, 128 ** -0.5, 2.0 ** -32)
+    tol = (2 * ds + 2.0 ** -11 + 2.0 ** -21 + 200 * 2.0 ** -23) * spread + tiny
+    tol = tol + _half_step(want.abs() + tol, q.dtype)
+    assert ((O.double() - want).abs() <= tol).all()
 
 
 def test_scale_argument_and_wide_values(rb, cuda):
