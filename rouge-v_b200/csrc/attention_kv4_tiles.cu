@@ -8,7 +8,7 @@
 //                   has grown by more than 2^8
 //   warps 8-11      one thread per key: codes from the pages to f16 K and V
 //                   rows in shared memory (128-byte swizzle), one block ahead
-//   warp 12         issues S = Q K^T (operands in shared memory) and O += P V
+//   warp 12         (its warpgroup idle otherwise) issues S = Q K^T (operands in shared memory) and O += P V
 //                   (P in TMEM, V as it lies: keys x d, the N-major operand)
 //
 // While one tile's softmax runs, the tensor cores work on the other. The
@@ -33,12 +33,25 @@
 namespace rb200 {
 namespace {
 
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;
+// Registers per thread of the warpgroups, from a launch with 128 each: the
+// softmax threads hold a whole row of scores (2 x 192 + 88 + 40 = 4 x 128).
+constexpr int kSoftmaxRegs = 192, kRowRegs = 88, kIssueRegs = 40;
+static_assert(2 * kSoftmaxRegs + kRowRegs + kIssueRegs == 4 * 128, "registers of the launch");
 constexpr int kKeys = 128;           // per block of keys
 constexpr int kRows = 256;           // per CTA
 constexpr uint32_t kChunk = 16384;   // 128 rows x 128 bytes (64 f16)
 constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
 constexpr float kTop = 7.0f;         // weights are held times 2^7: at most 2^15
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int DH>
 struct TileCfg {
@@ -154,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
+    more_registers<kSoftmaxRegs>();
     const int w = warp >> 2, tr = threadIdx.x & 127;  // tile, row in it
     const int r = r0 + w * 128 + tr;
     const bool live = r < nrows;
@@ -203,25 +217,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       tc_fence_after_sync();
       const int key0 = first + j * kKeys;
       const bool whole = __all_sync(0xffffffffu, key0 >= col_lo && key0 + kKeys <= col_hi);
-      uint32_t x[2][32];
-      float m = -INFINITY;
-      tmem_ld_32x32b_x32(s_t, x[0]);
+      uint32_t x[4][32];  // the row's scores
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait_regs(x[c & 1]);
-        if (c < 3) tmem_ld_32x32b_x32(s_t + 32 * (c + 1), x[(c + 1) & 1]);
-        if (whole) {
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_t + 32 * c, x[c]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            m = max3(m, __uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1]));
-        } else {
+      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(x[c]);
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int key = key0 + 32 * c + i;
-            if (key >= col_lo && key < col_hi) m = fmaxf(m, __uint_as_float(x[c & 1][i]));
+            if (key < col_lo || key >= col_hi) x[c][i] = 0xFF800000u;  // -inf
           }
-        }
       }
+      float mm[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mm[c] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          mm[c] = max3(mm[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+      }
+      const float m = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3]));
       const float logit = m * mult;
       const bool grow = logit > top + kGrow;  // (the first keys of a row always)
       if (__any_sync(0xffffffffu, grow)) {
@@ -241,29 +259,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
         }
       }
       const float off = top == -INFINITY ? 0.0f : kTop - top;
-      tmem_ld_32x32b_x32(s_t, x[0]);
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait_regs(x[c & 1]);
-        if (c < 3) tmem_ld_32x32b_x32(s_t + 32 * (c + 1), x[(c + 1) & 1]);
         uint32_t h[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float u0 = __uint_as_float(x[c & 1][i]), u1 = __uint_as_float(x[c & 1][i + 1]);
-          if (!whole) {
-            const int key = key0 + 32 * c + i;
-            if (key < col_lo || key >= col_hi) u0 = -INFINITY;
-            if (key + 1 < col_lo || key + 1 >= col_hi) u1 = -INFINITY;
-          }
-          u0 = ex2(__fmaf_rn(u0, mult, off));
-          u1 = ex2(__fmaf_rn(u1, mult, off));
-          sum += u0 + u1;
+          float u0, u1;
+          fma2(u0, u1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mult, off, off);
+          u0 = ex2(u0);
+          u1 = ex2(u1);
+          part[(i >> 1) & 3] += u0 + u1;
           h[i / 2] = f16x2_rn(u0, u1);
         }
-        // (weights of keys 32c .. lie over scores that this lane has read:
-        // columns 16c .. 16c + 15; chunk c + 1, still on its way, is behind)
-        tmem_st_32x32b_x16(s_t + 16 * c, h);
+        tmem_st_32x32b_x16(s_t + 16 * c, h);  // (over the scores, which are in registers)
       }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(&p_full[w]);
@@ -299,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ K and V rows
+    fewer_registers<kRowRegs>();
     const int kr = threadIdx.x - 256;
     const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
     KeyRow<DH> k, v;
@@ -337,8 +349,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       mbar_arrive(&v_full[s]);
       fetch(j + 1);
     }
-  } else if (lane == 0 && blocks > 0) {
+  } else {
     // ------------------------------------------------------------ MMA issuer
+    fewer_registers<kIssueRegs>();
+    if (warp == 12 && lane == 0 && blocks > 0) {
     const uint32_t id_s = make_idesc(1u, 0u, 0u, 0u, 0u, 128, kKeys);
     const uint32_t id_o = make_idesc(1u, 0u, 0u, 0u, 1u, 128, DH);
     bool issued = false;
@@ -389,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
         tc_commit(drain);
         mbar_wait(drain, 0, &never);
       }
+    }
     }
   }
   tc_fence_before_sync();
