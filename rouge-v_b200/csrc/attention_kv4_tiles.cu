@@ -3,18 +3,23 @@
 // the tcgen05 tensor cores, 128 keys at a time.
 //
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: one thread per row. Scores
-//                   from TMEM, running maximum and sum, weights as f16 back
-//                   to TMEM (over the scores), O rescaled when the maximum
-//                   has grown by more than 2^8
+//                   of 64 keys from TMEM, running maximum and sum, weights
+//                   as f16 back to TMEM (over the scores), O rescaled when
+//                   the maximum has grown by more than 2^8
 //   warps 8-11      one thread per key: codes from the pages to f16 K and V
 //                   rows in shared memory (128-byte swizzle), one block ahead
-//   warp 12         (its warpgroup idle otherwise) issues S = Q K^T (operands in shared memory) and O += P V
-//                   (P in TMEM, V as it lies: keys x d, the N-major operand)
+//   warps 12, 13    issue tile 0's and 1's S = Q K^T (operands in shared
+//                   memory) and O += P V (P in TMEM, V as it lies: keys x d,
+//                   the N-major operand)
 //
-// While one tile's softmax runs, the tensor cores work on the other. The
-// scores' columns hold the weights afterwards, so a tile's next S is issued
-// when its O += P V has completed; a tile's S in hand thus also means that
-// its O is up to date and may be rescaled.
+// A tile's scores are two halves of 64 keys (TMEM holds two tiles' scores and
+// two O of 128 columns each): while one half is in the softmax, the tensor
+// cores multiply the other half's weights by V and form its next scores. A
+// half's columns hold its weights afterwards, so its next scores are issued
+// when its O += P V has completed; two issuing threads, because each such
+// group of MMAs takes 340 cycles to start and to be seen done, which the
+// other tile's fill. (One half of 128 keys and one issuer: 4900 cycles per
+// block of 128 keys, against 6400 with the scores read twice.)
 //
 // What bounds it: per 128 x 128 block of one tile at Dh 128 the two products
 // take 1024 cycles at the measured matrix rate, the 16384 exponentials as
@@ -33,25 +38,13 @@
 namespace rb200 {
 namespace {
 
-constexpr int kThreads = 16 * 32;
-// Registers per thread of the warpgroups, from a launch with 128 each: the
-// softmax threads hold a whole row of scores (2 x 192 + 88 + 40 = 4 x 128).
-constexpr int kSoftmaxRegs = 192, kRowRegs = 88, kIssueRegs = 40;
-static_assert(2 * kSoftmaxRegs + kRowRegs + kIssueRegs == 4 * 128, "registers of the launch");
-constexpr int kKeys = 128;           // per block of keys
+constexpr int kThreads = 14 * 32;
+constexpr int kKeys = 128;           // per block of K and V
+constexpr int kHalf = 64;            // per step of the softmax
 constexpr int kRows = 256;           // per CTA
 constexpr uint32_t kChunk = 16384;   // 128 rows x 128 bytes (64 f16)
 constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
 constexpr float kTop = 7.0f;         // weights are held times 2^7: at most 2^15
-
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 template <int DH>
 struct TileCfg {
@@ -115,10 +108,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
                                               ~static_cast<uintptr_t>(1023));
   const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * C::TILE, v_s = k_s + 2 * C::TILE;
   uint64_t *bar = reinterpret_cast<uint64_t *>(smem + 6 * C::TILE);
-  uint64_t *q_full = bar, *k_full = bar + 1, *v_full = bar + 3, *k_empty = bar + 5, *v_empty = bar + 7,
-           *s_full = bar + 9, *p_full = bar + 11, *pv_done = bar + 13, *drain = bar + 15;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 16);
-  volatile int *abort = reinterpret_cast<volatile int *>(bar + 17);
+  // [tile]; [stage]; [tile][half]
+  uint64_t *q_full = bar, *k_full = bar + 2, *v_full = bar + 4, *k_empty = bar + 6, *v_empty = bar + 8,
+           *s_full = bar + 10, *p_full = bar + 14, *pv_done = bar + 18, *drain = bar + 22;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 24);
+  volatile int *abort = reinterpret_cast<volatile int *>(bar + 25);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // unit: the last row tiles, which see the most keys, first
@@ -135,20 +129,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
   const int hi_max = a.causal ? max(0, min(len, p0 + r1 / a.group + 1)) : len;
   const int lo_min = a.window > 0 ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
   const int first = lo_min / kKeys * kKeys;
-  const int blocks = hi_max > first ? (hi_max - first + kKeys - 1) / kKeys : 0;
+  const int steps = hi_max > first ? (hi_max - first + kHalf - 1) / kHalf : 0;
+  const int blocks = (steps + 1) / 2;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, kRows);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
       mbar_init(&k_full[i], 128);
       mbar_init(&v_full[i], 128);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&k_empty[i], 2);  // (one commit of each tile's issuer)
+      mbar_init(&v_empty[i], 2);
+      mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(drain, 1);
     *abort = 0;
     mbar_init_fence();
   }
@@ -167,7 +164,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    more_registers<kSoftmaxRegs>();
     const int w = warp >> 2, tr = threadIdx.x & 127;  // tile, row in it
     const int r = r0 + w * 128 + tr;
     const bool live = r < nrows;
@@ -202,58 +198,57 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
         st_shared_v4(q_s + w * C::TILE + unit_at(tr, 2 * k + 1), h[4], h[5], h[6], h[7]);
       }
       fence_async_smem();
-      mbar_arrive(q_full);
+      mbar_arrive(&q_full[w]);
     }
     const uint32_t row_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem + w * 128 + row_lane, o_t = tmem + C::O_COL + w * DH + row_lane;
     float top = -INFINITY, sum = 0.0f;
     bool ok = true;
-    for (int j = 0; j < blocks; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[w], j & 1, abort));
-      if (!ok) {
-        if (lane == 0) fail();
-        break;
-      }
+    for (int i = 0; i < steps; ++i) {
+      const int h = i & 1, j = i >> 1;
+      const uint32_t s_h = s_t + kHalf * h;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * w + h], j & 1, abort));
+      if (!ok) break;
       tc_fence_after_sync();
-      const int key0 = first + j * kKeys;
-      const bool whole = __all_sync(0xffffffffu, key0 >= col_lo && key0 + kKeys <= col_hi);
-      uint32_t x[4][32];  // the row's scores
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_t + 32 * c, x[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(x[c]);
+      uint32_t x[2][32];  // the row's scores
+      tmem_ld_32x32b_x32(s_h, x[0]);
+      tmem_ld_32x32b_x32(s_h + 32, x[1]);
+      const int key0 = first + i * kHalf;
+      const bool whole = __all_sync(0xffffffffu, key0 >= col_lo && key0 + kHalf <= col_hi);
+      tmem_ld_wait_regs(x[0]);
+      tmem_ld_wait_regs(x[1]);
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int key = key0 + 32 * c + i;
-            if (key < col_lo || key >= col_hi) x[c][i] = 0xFF800000u;  // -inf
+          for (int k = 0; k < 32; ++k) {
+            const int key = key0 + 32 * c + k;
+            if (key < col_lo || key >= col_hi) x[c][k] = 0xFF800000u;  // -inf
           }
       }
-      float mm[4];
+      float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mm[c] = -INFINITY;
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          mm[c] = max3(mm[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-      }
-      const float m = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3]));
-      const float logit = m * mult;
+        for (int k = 0; k < 32; k += 2)
+          mm[(k >> 1) & 3] = max3(mm[(k >> 1) & 3], __uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1]));
+      const float logit = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * mult;
       const bool grow = logit > top + kGrow;  // (the first keys of a row always)
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? ex2(top - logit) : 1.0f;
         if (grow) top = logit;
         sum *= f;
-        if (j > 0) {
+        if (i > 0) {  // the last O += P V done, then O times f
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[2 * w + (h ^ 1)], ((i - 1) >> 1) & 1, abort));
+          if (!ok) break;
+          tc_fence_after_sync();
 #pragma unroll 1
           for (int c = 0; c < DH / 16; ++c) {
             uint32_t y[16];
             tmem_ld_32x32b_x16(o_t + 16 * c, y);
             tmem_ld_wait_regs16(y);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
             tmem_st_32x32b_x16(o_t + 16 * c, y);
           }
         }
@@ -261,36 +256,37 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       const float off = top == -INFINITY ? 0.0f : kTop - top;
       float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t h[16];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int k = 0; k < 32; k += 2) {
           float u0, u1;
-          fma2(u0, u1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mult, off, off);
+          fma2(u0, u1, __uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1]), mult, off, off);
           u0 = ex2(u0);
           u1 = ex2(u1);
-          part[(i >> 1) & 3] += u0 + u1;
-          h[i / 2] = f16x2_rn(u0, u1);
+          part[(k >> 1) & 3] += u0 + u1;
+          p[k / 2] = f16x2_rn(u0, u1);
         }
-        tmem_st_32x32b_x16(s_t + 16 * c, h);  // (over the scores, which are in registers)
+        tmem_st_32x32b_x16(s_h + 16 * c, p);  // (over the scores, which are in registers)
       }
       sum += (part[0] + part[1]) + (part[2] + part[3]);
       tmem_st_wait();
       tc_fence_before_sync();
-      mbar_arrive(&p_full[w]);
+      mbar_arrive(&p_full[2 * w + h]);
     }
-    if (ok && blocks > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[w], (blocks - 1) & 1, abort));
-      if (!ok && lane == 0) fail();
+    if (ok && steps > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[2 * w + ((steps - 1) & 1)],
+                                             ((steps - 1) >> 1) & 1, abort));
       tc_fence_after_sync();
     }
+    if (!ok && lane == 0) fail();
     if (ok) {
       const float gv = a.gs_v ? __ldg(a.gs_v + hk) : 1.0f;
       const float f = sum > 0.0f || sum != sum ? gv / sum : 0.0f;
 #pragma unroll 1
       for (int c = 0; c < DH / 32; ++c) {
         uint32_t y[32];
-        if (blocks > 0) {
+        if (steps > 0) {
           tmem_ld_32x32b_x32(o_t + 32 * c, y);
           tmem_ld_wait_regs(y);
         } else {
@@ -310,7 +306,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ K and V rows
-    fewer_registers<kRowRegs>();
     const int kr = threadIdx.x - 256;
     const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
     KeyRow<DH> k, v;
@@ -349,49 +344,47 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       mbar_arrive(&v_full[s]);
       fetch(j + 1);
     }
-  } else {
-    // ------------------------------------------------------------ MMA issuer
-    fewer_registers<kIssueRegs>();
-    if (warp == 12 && lane == 0 && blocks > 0) {
-    const uint32_t id_s = make_idesc(1u, 0u, 0u, 0u, 0u, 128, kKeys);
+  } else if (lane == 0 && steps > 0) {
+    // ------------------------------------------------------------ MMA issuers
+    const int w = warp - 12;
+    const uint32_t id_s = make_idesc(1u, 0u, 0u, 0u, 0u, 128, kHalf);
     const uint32_t id_o = make_idesc(1u, 0u, 0u, 0u, 1u, 128, DH);
     bool issued = false;
-    auto scores = [&](int w, int s) {  // S_w = Q_w K_s^T
+    auto scores = [&](int i) {  // S of step i: Q_w K^T for its 64 keys
+      const int h = i & 1, s = (i >> 1) & 1;
 #pragma unroll
       for (int k = 0; k < DH / 16; ++k) {
         const uint32_t step = (k >> 2) * kChunk + (k & 3) * 32;
-        umma<MmaKind::F16>(tmem + w * 128, smem_desc_sw128(q_s + w * C::TILE + step, 16, 1024),
-                           smem_desc_sw128(k_s + s * C::TILE + step, 16, 1024), id_s, k != 0);
+        umma<MmaKind::F16>(tmem + w * 128 + kHalf * h, smem_desc_sw128(q_s + w * C::TILE + step, 16, 1024),
+                           smem_desc_sw128(k_s + s * C::TILE + step + h * kHalf * 128, 16, 1024), id_s,
+                           k != 0);
       }
-      tc_commit(&s_full[w]);
+      tc_commit(&s_full[2 * w + h]);
+      if (h == 1 || i == steps - 1) tc_commit(&k_empty[s]);  // the block's last scores
       issued = true;
     };
     auto run = [&]() {
-      if (!mbar_wait(q_full, 0, abort) || !mbar_wait(&k_full[0], 0, abort)) return false;
+      if (!mbar_wait(&q_full[w], 0, abort) || !mbar_wait(&k_full[0], 0, abort)) return false;
       tc_fence_after_sync();
-      scores(0, 0);
-      scores(1, 0);
-      tc_commit(&k_empty[0]);
-      for (int j = 0; j < blocks; ++j) {
-        const int s = j & 1, sn = s ^ 1;
-        for (int w = 0; w < 2; ++w) {
-          if (!mbar_wait(&p_full[w], j & 1, abort)) return false;
-          if (w == 0 && !mbar_wait(&v_full[s], (j >> 1) & 1, abort)) return false;
-          tc_fence_after_sync();
+      scores(0);
+      if (steps > 1) scores(1);
+      for (int i = 0; i < steps; ++i) {
+        const int h = i & 1, j = i >> 1, s = j & 1;
+        if (!mbar_wait(&p_full[2 * w + h], j & 1, abort)) return false;
+        if (h == 0 && !mbar_wait(&v_full[s], (j >> 1) & 1, abort)) return false;
+        tc_fence_after_sync();
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_f16_ta(tmem + C::O_COL + w * DH, tmem + w * 128 + 8 * k,
-                        smem_desc_sw128(v_s + s * C::TILE + k * 16 * 128, kChunk, 1024), id_o,
-                        (j | k) != 0);
-          tc_commit(&pv_done[w]);
-          if (w == 1) tc_commit(&v_empty[s]);
-          if (j + 1 < blocks) {
-            if (w == 0 && !mbar_wait(&k_full[sn], ((j + 1) >> 1) & 1, abort)) return false;
-            if (!mbar_wait(&pv_done[w], j & 1, abort)) return false;
-            tc_fence_after_sync();
-            scores(w, sn);
-            if (w == 1) tc_commit(&k_empty[sn]);
-          }
+        for (int k = 0; k < kHalf / 16; ++k)
+          umma_f16_ta(tmem + C::O_COL + w * DH, tmem + w * 128 + kHalf * h + 8 * k,
+                      smem_desc_sw128(v_s + s * C::TILE + (h * kHalf + k * 16) * 128, kChunk, 1024), id_o,
+                      (i | k) != 0);
+        tc_commit(&pv_done[2 * w + h]);
+        if (h == 1 || i == steps - 1) tc_commit(&v_empty[s]);  // the block's last use
+        if (i + 2 < steps) {
+          if (h == 0 && !mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort)) return false;
+          if (!mbar_wait(&pv_done[2 * w + h], j & 1, abort)) return false;
+          tc_fence_after_sync();
+          scores(i + 2);
         }
       }
       return true;
@@ -400,10 +393,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       fail();
       if (issued) {  // the MMAs already issued complete before TMEM is released
         const volatile int never = 0;
-        tc_commit(drain);
-        mbar_wait(drain, 0, &never);
+        tc_commit(&drain[w]);
+        mbar_wait(&drain[w], 0, &never);
       }
-    }
     }
   }
   tc_fence_before_sync();
