@@ -61,7 +61,7 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) 
   if (a.window > 0) lo = max(0, min(s.len, s.p0 - a.window + 1));
   s.lo_tile = lo / kTile;
   s.tiles = max(1, (s.len + kTile - 1) / kTile - s.lo_tile);
-  s.rts = (s.nq * a.group + rows - 1) / rows;
+  s.rts = (s.nq * a.group + rows - 1) / rows;  // (rows is 8 or 16)
   s.work = static_cast<long long>(s.tiles) * s.rts * a.Hkv;
   return s;
 }
@@ -70,6 +70,29 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) 
 __device__ __forceinline__ long long divide(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
   return a / b;
+}
+
+// The sequence that lane l of the warp holds.
+__device__ __forceinline__ SeqInfo seq_of_lane(const SeqInfo &m, int l) {
+  SeqInfo s;
+  s.nq = __shfl_sync(0xffffffffu, m.nq, l);
+  s.len = __shfl_sync(0xffffffffu, m.len, l);
+  s.q0 = __shfl_sync(0xffffffffu, m.q0, l);
+  s.p0 = __shfl_sync(0xffffffffu, m.p0, l);
+  s.tiles = __shfl_sync(0xffffffffu, m.tiles, l);
+  s.rts = __shfl_sync(0xffffffffu, m.rts, l);
+  s.lo_tile = __shfl_sync(0xffffffffu, m.lo_tile, l);
+  s.work = __shfl_sync(0xffffffffu, m.work, l);
+  return s;
+}
+
+__device__ __forceinline__ long long inclusive_scan(long long v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -134,50 +157,55 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
   const int gw = warp * gridDim.x + blockIdx.x;  // (few warps: one per SM)
   grid_launch_dependents();
 
-  // total work
-  {
+  if (lane == 0) {
+    for (int s = 0; s < S::STAGES; ++s) mbar_init(&full[warp][s], 1);
+    mbar_init_fence();
+  }
+  // sequences b0 .. b0 + 31, one per lane; total work
+  int b0 = 0;
+  SeqInfo mine{};
+  auto hold = [&](int base) {
+    b0 = base;
+    mine = SeqInfo{};
+    if (base + lane < a.B) mine = seq_info(a, base + lane, S::ROWS);
+  };
+  hold(0);
+  long long inc = inclusive_scan(mine.work, lane);
+  long long total = __shfl_sync(0xffffffffu, inc, 31);
+  if (a.B > 32) {  // (the block adds up the others)
     long long w = 0;
-    for (int b = threadIdx.x; b < a.B; b += kWarps * 32) w += seq_info(a, b, S::ROWS).work;
+    for (int b = 32 + threadIdx.x; b < a.B; b += kWarps * 32) w += seq_info(a, b, S::ROWS).work;
 #pragma unroll
     for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     if (lane == 0) total_slot[warp] = w;
-    if (lane == 0)
-      for (int s = 0; s < S::STAGES; ++s) mbar_init(&full[warp][s], 1);
-    mbar_init_fence();
-  }
-  __syncthreads();
-  long long total = 0;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) total += total_slot[i];
+    for (int i = 0; i < kWarps; ++i) total += total_slot[i];
+  }
   // active warps, and this warp's range of tiles
   long long active = total >> kMinTilesLog2;
   active = active < 1 ? 1 : (active > a.warps ? a.warps : active);
   const long long share = divide(total, active), rest = total - share * active;
   long long pos = gw * share + (gw < rest ? gw : rest);
   const long long pos_end = gw < active ? pos + share + (gw < rest ? 1 : 0) : pos;
-  if (lane < 2) a.desc[2 * gw + lane] = make_int4(0, 0, 0, 0);
-  __syncwarp();
+  if (!a.by_unit && lane == 0) a.joins[gw] = make_int4(0, 0, 0, 0);
   if (pos >= pos_end) return;
+  __syncwarp();
 
-  // sequence that holds `pos`: warp scans of 32 sequences
+  // sequence that holds `pos`
   int b = 0;
   long long before = 0;  // work before sequence b
-  for (int b0 = 0;; b0 += 32) {
-    const long long w = b0 + lane < a.B ? seq_info(a, b0 + lane, S::ROWS).work : 0;
-    long long inc = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
-    }
+  for (;;) {
     const unsigned past = __ballot_sync(0xffffffffu, before + inc > pos);
     if (past) {
       const int l = __ffs(past) - 1;
       b = b0 + l;
-      before += __shfl_sync(0xffffffffu, inc - w, l);
+      before += __shfl_sync(0xffffffffu, inc - mine.work, l);
       break;
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
+    hold(b0 + 32);
+    inc = inclusive_scan(mine.work, lane);
   }
 
   const int Dh = FULL ? DT : a.Dh;
@@ -198,7 +226,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
   uint32_t parity = 0;       // of s_out's barrier
   bool alive = true;
 
-  SeqInfo si = seq_info(a, b, S::ROWS);
+  SeqInfo si = seq_of_lane(mine, b - b0);
   while (alive && pos < pos_end) {
     while (pos >= before + si.work) {  // next sequence
       before += si.work;
@@ -208,9 +236,10 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     const long long in_seq = pos - before;
     const int unit = static_cast<int>(divide(in_seq, si.tiles));
     const int first = static_cast<int>(in_seq - static_cast<long long>(unit) * si.tiles);
-    const int hk = unit % a.Hkv, rt = unit / a.Hkv;
+    const int rt = a.by_heads.div(unit), hk = unit - rt * a.Hkv;
     const long long left = pos_end - pos;
     const int last = left < si.tiles - first ? first + static_cast<int>(left) : si.tiles;
+    const long long unit_end = pos + (si.tiles - first);
     pos += last - first;
     const bool whole = first == 0 && last == si.tiles;
 
@@ -218,8 +247,9 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     const int r0 = rt * S::ROWS, nrows = si.nq * a.group;
     const int r1 = min(r0 + S::ROWS, nrows) - 1;
     const int p0 = si.p0;
-    const int hi_max = a.causal ? max(0, min(si.len, p0 + r1 / a.group + 1)) : si.len;
-    const int lo_min = a.window > 0 ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
+    auto q_of = [&](int r) { return static_cast<int>(a.by_group.div(r)); };  // query of a row
+    const int hi_max = a.causal ? max(0, min(si.len, p0 + q_of(r1) + 1)) : si.len;
+    const int lo_min = a.window > 0 ? max(0, p0 + q_of(r0) - a.window + 1) : 0;
     int col_lo[S::NR][2], col_hi[S::NR][2];
     int hi_min = 0x7fffffff, lo_max = 0;
 #pragma unroll
@@ -227,14 +257,29 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = r0 + j * 8 + 2 * t + e;
-        const int p = p0 + r / a.group;
+        const int p = p0 + q_of(r);
         col_hi[j][e] = r < nrows ? (a.causal ? min(si.len, p + 1) : si.len) : si.len;
         col_lo[j][e] = a.window > 0 && r < nrows ? max(0, p - a.window + 1) : 0;
       }
-    hi_min = a.causal ? min(si.len, p0 + r0 / a.group + 1) : si.len;
-    lo_max = a.window > 0 ? max(0, p0 + r1 / a.group - a.window + 1) : 0;
+    hi_min = a.causal ? min(si.len, p0 + q_of(r0) + 1) : si.len;
+    lo_max = a.window > 0 ? max(0, p0 + q_of(r1) - a.window + 1) : 0;
     const int t_lo = max(si.lo_tile + first, lo_min / kTile);
     const int t_hi = min(si.lo_tile + last, (hi_max + kTile - 1) / kTile);
+
+    // ---- this lane's part of its query rows, on its way while the copies start
+    RawQ<T> raw[S::NR][kBlk];
+#pragma unroll
+    for (int j = 0; j < S::NR; ++j) {
+      const int r = r0 + j * 8 + g, i = q_of(r);
+      const long long at =
+          (static_cast<long long>(si.q0 + i) * a.Hq + hk * a.group + (r - i * a.group)) * Dh;
+#pragma unroll
+      for (int k = 0; k < kBlk; ++k) {
+        const int d = t * (DT / 4) + 16 * k;
+        raw[j][k].zero();
+        if (r < nrows && (FULL || d < Dh)) raw[j][k].load(a.Q, at + d);
+      }
+    }
 
     // ---- copies: half tiles of 16 keys, each within one page. Lane l of the
     // first eight copies array l / 2 (K codes, V codes, K scales, V scales),
@@ -246,7 +291,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     auto half_row = [&](int half) {
       const int key = half * 16;
       if (key >= hi_max || key + 16 <= lo_min) return kNone;  // (no row's keys)
-      const int pi = key / a.page;
+      const int pi = a.by_page.div(key);
       const int id = pi < a.max_pages ? __ldg(table + pi) : -1;
       if (id < 0 || id >= a.pages) {
         atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
@@ -286,22 +331,10 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
       const float gk = a.gs_k ? __ldg(a.gs_k + hk) : 1.0f;
 #pragma unroll
       for (int j = 0; j < S::NR; ++j) {
-        const int r = r0 + j * 8 + g;
-        const bool live = r < nrows;
-        const int qi = si.q0 + (live ? r / a.group : 0), h = hk * a.group + (live ? r % a.group : 0);
-        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh;
         float v[DT / 4];
         float m = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kBlk; ++k) {
-          const int d = t * (DT / 4) + 16 * k;
-          if (live && (FULL || d < Dh)) {
-            load_q16<T>(a.Q, at + d, v + 16 * k);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[16 * k + i] = 0.0f;
-          }
-        }
+        for (int k = 0; k < kBlk; ++k) raw[j][k].unpack(v + 16 * k);
 #pragma unroll
         for (int k = 0; k < DT / 4; ++k) m = fmaxf(m, fabsf(v[k]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -585,7 +618,16 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     const float gv = a.gs_v ? __ldg(a.gs_v + hk) : 1.0f;
     const int slot = 2 * gw + (first == 0 ? 1 : 0);
     float *part = a.part + static_cast<size_t>(slot) * S::ROWS * (Dh + 4);
-    if (!whole && lane == 0) a.desc[slot] = make_int4(b, hk, rt, 1);
+    if (first == 0 && lane == 0) {
+      // how many warps share the unit: the one that holds its last tile
+      const long long e = unit_end - 1, long_end = rest * (share + 1);
+      const long long w1 = e < long_end ? divide(e, share + 1) : rest + divide(e - long_end, share);
+      const int n = static_cast<int>(w1) - gw + 1;
+      if (a.by_unit)
+        a.joins[(b * a.row_tiles + rt) * a.Hkv + hk] = make_int4(b, unit, gw, n);
+      else if (n > 1)
+        a.joins[gw] = make_int4(b, unit, gw, n);
+    }
 #pragma unroll
     for (int j = 0; j < S::NR; ++j)
 #pragma unroll
@@ -597,16 +639,17 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         const int rr = j * 8 + 2 * t + e, r = r0 + rr;
         if (r >= nrows) continue;
         const float f = whole ? (l > 0.0f || l != l ? gv / l : 0.0f) : 1.0f;
-        const int qi = si.q0 + r / a.group, h = hk * a.group + r % a.group;
-        const long long at = (static_cast<long long>(qi) * a.Hq + h) * Dh + g * (DT / 8);
+        const int i = q_of(r);
+        const long long at =
+            (static_cast<long long>(si.q0 + i) * a.Hq + hk * a.group + (r - i * a.group)) * Dh + g * (DT / 8);
 #pragma unroll
         for (int m = 0; m < kMt; m += 2) {  // values g * DT / 8 + 2m .. + 3
           if (!FULL && g * (DT / 8) + 2 * m >= Dh) continue;
           float v[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = o[j][m + i / 2][2 * (i & 1) + e];
-            if constexpr (S::SPLIT) v[i] += o[S::NR + j][m + i / 2][2 * (i & 1) + e];
+          for (int k = 0; k < 4; ++k) {
+            v[k] = o[j][m + k / 2][2 * (k & 1) + e];
+            if constexpr (S::SPLIT) v[k] += o[S::NR + j][m + k / 2][2 * (k & 1) + e];
           }
           if (whole)
             store_o4<T>(a.O, at + 2 * m, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
@@ -622,10 +665,13 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
   }
 }
 
-// Joins the parts of the units that several warps computed: block (w, y)
-// handles the unit whose first part is slot 2w + 1 -- the others are the
-// first slots of the warps after it -- and, of its rows, the y-th of
-// gridDim.y shares. Order and so rounding are fixed.
+// Joins the parts of the units that several warps computed. joins holds, per
+// unit that n warps from w0 on share, {sequence, row tile and head, w0, n}:
+// by unit where there are fewer units than warps (an entry is valid if the
+// unit has rows), else by w0 (n = 0: none). The first part is slot 2 w0 + 1,
+// the others the first slots of the warps after it. A block joins a unit's
+// rows, or the y-th of gridDim.y shares of them. Order and so rounding are
+// fixed.
 constexpr int kJoinThreads = 256;
 
 template <int T>
@@ -633,29 +679,29 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
   __shared__ float4 acc[kJoinThreads];
   __shared__ float weight_sum[kJoinThreads];
   __shared__ float row_max[16];
+  const int tid = threadIdx.x;
+  int b = 0, rt = 0, hk = 0;
+  if (a.by_unit) {
+    const int seq_tile = a.by_heads.div(blockIdx.x);
+    hk = blockIdx.x - seq_tile * a.Hkv;
+    b = a.by_tiles.div(seq_tile);
+    rt = seq_tile - b * a.row_tiles;
+  }
   grid_dependency_wait();
-  const int w0 = blockIdx.x, tid = threadIdx.x;
-  const int4 u = a.desc[2 * w0 + 1];
-  if (!u.w) return;
-  const int q0 = a.cu_q ? a.cu_q[u.x] : u.x;
-  int nq = a.cu_q ? a.cu_q[u.x + 1] - q0 : 1;
+  const int4 u = __ldcg(a.joins + blockIdx.x);
+  if (!a.by_unit) {
+    if (u.w < 2) return;
+    b = u.x;
+    rt = a.by_heads.div(u.y);
+    hk = u.y - rt * a.Hkv;
+  }
+  const int q0 = a.cu_q ? a.cu_q[b] : b;
+  int nq = a.cu_q ? a.cu_q[b + 1] - q0 : 1;
   nq = max(0, min(nq, a.max_q));
   const int share = rows / gridDim.y, first = blockIdx.y * share;
-  const int live = min(share, nq * a.group - u.z * rows - first);  // this block's rows
-  if (live <= 0) return;
-  // parts of the unit: the first slots of w0 + 1 .. that carry it
-  int n = 1;
-  for (;;) {
-    const int i = w0 + n + tid;
-    bool same = false;
-    if (i < a.warps) {
-      const int4 d = a.desc[2 * i];
-      same = d.w && d.x == u.x && d.y == u.y && d.z == u.z;
-    }
-    const int c = __syncthreads_count(same);
-    n += c;
-    if (c < kJoinThreads) break;
-  }
+  const int live = min(share, nq * a.group - rt * rows - first);  // this block's rows
+  if (live <= 0 || u.w < 2) return;
+  const int w0 = u.z, n = u.w;
   const size_t stride = static_cast<size_t>(rows) * (a.Dh + 4);
   auto part = [&](int i) { return a.part + (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * stride; };
   for (int r = tid >> 5; r < live; r += kJoinThreads / 32) {
@@ -670,7 +716,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
   const int lanes = a.Dh / 4, per_row = kJoinThreads / lanes;
   const int rows_at_once = live < per_row ? live : per_row, groups = per_row / rows_at_once;
   const int d = (tid % lanes) * 4, slot = tid / lanes;
-  const float gv = a.gs_v ? a.gs_v[u.y] : 1.0f;
+  const float gv = a.gs_v ? a.gs_v[hk] : 1.0f;
   for (int r0 = 0; r0 < live; r0 += rows_at_once) {
     const int r = r0 + slot % rows_at_once, grp = slot / rows_at_once;
     const bool on = grp < groups && r < live && slot < per_row;
@@ -699,9 +745,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
         l += weight_sum[o];
       }
       const float f = (l > 0.0f || l != l) ? gv / l : 0.0f;
-      const int row = u.z * rows + rr;
+      const int row = rt * rows + rr, q = a.by_group.div(row);
       const long long at =
-          (static_cast<long long>(q0 + row / a.group) * a.Hq + u.y * a.group + row % a.group) * a.Dh + d;
+          (static_cast<long long>(q0 + q) * a.Hq + hk * a.group + (row - q * a.group)) * a.Dh + d;
       store_o4<T>(a.O, at, v.x * f, v.y * f, v.z * f, v.w * f);
     }
   }
@@ -751,7 +797,7 @@ int launch_kernels(const AttnArgs &a, int join_y, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.warps, join_y, 1);
+  cfg.gridDim = dim3(a.by_unit ? a.B * a.Hkv * a.row_tiles : a.warps, join_y, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = st;
   cfg.attrs = attr;
@@ -763,9 +809,7 @@ template <int DT, int NT, int T>
 int launch_shape(const AttnArgs &a, cudaStream_t st) {
   // A block joins all rows of a unit, or, where a unit may be cut into more
   // than 16 parts (few units), one row.
-  const double units = static_cast<double>(a.B) * a.Hkv *
-                       ((static_cast<double>(a.max_q) * a.group + Shape<DT, NT, T>::ROWS - 1) /
-                        Shape<DT, NT, T>::ROWS);
+  const double units = static_cast<double>(a.B) * a.Hkv * a.row_tiles;
   const int join_y = a.warps > 16 * units ? Shape<DT, NT, T>::ROWS : 1;
   return a.Dh == DT ? launch_kernels<DT, NT, T, true>(a, join_y, st)
                     : launch_kernels<DT, NT, T, false>(a, join_y, st);
@@ -797,7 +841,7 @@ size_t rouge_b200_attention_kv4_workspace(int B, int Hq, int Hkv, int Dh, int ma
       max_kv <= 0 || !valid_float_type(type) || device_ready() != ROUGE_B200_OK)
     return 0;
   const int warps = grid_warps(B, Hkv, Hq / Hkv, Dh, max_q, max_kv, type);
-  return part_bytes(warps, rows_of(Hq / Hkv, max_q, type), Dh) + static_cast<size_t>(2) * warps * 16;
+  return part_bytes(warps, rows_of(Hq / Hkv, max_q, type), Dh) + static_cast<size_t>(warps) * 16;
 }
 
 int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type, int B, int Hq,
@@ -831,10 +875,16 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   const int rt_rows = rows_of(a.group, max_q, type);
   a.warps = grid_warps(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type);
   const size_t pb = part_bytes(a.warps, rt_rows, a.Dh);
-  if (!workspace || workspace_bytes < pb + static_cast<size_t>(2) * a.warps * 16)
+  if (!workspace || workspace_bytes < pb + static_cast<size_t>(a.warps) * 16)
     return set_status(ROUGE_B200_ETOOBIG);
   a.part = static_cast<float *>(workspace);
-  a.desc = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + pb);
+  a.joins = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + pb);
+  a.row_tiles = static_cast<int>((rows + rt_rows - 1) / rt_rows);
+  a.by_unit = static_cast<double>(B) * a.Hkv * a.row_tiles < a.warps ? 1 : 0;
+  a.by_group = Divisor(a.group);
+  a.by_page = Divisor(a.page);
+  a.by_heads = Divisor(a.Hkv);
+  a.by_tiles = Divisor(a.row_tiles);
   a.err = device_error_word();
   if (!a.err) return set_status(ROUGE_B200_ENOMEM);
   cudaStream_t st = as_stream(stream);

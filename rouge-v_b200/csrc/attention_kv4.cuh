@@ -25,9 +25,12 @@ struct AttnArgs {
   int max_pages;
   float scale;
   int causal, window;
+  Divisor by_group, by_page, by_heads, by_tiles;  // (by_tiles: row tiles per sequence at most)
   int warps;      // warps of the grid
   float *part;    // [2 * warps][rows * (Dh + 4)]: weighted sums, then maximum and sum per row
-  int4 *desc;     // [2 * warps]: sequence, head, row tile, valid
+  int4 *joins;    // units that several warps share (see attention_kv4.cu)
+  int by_unit;    // joins is indexed by unit, not by warp
+  int row_tiles;  // row tiles of a sequence of max_q queries
   int *err;
 };
 
@@ -69,31 +72,45 @@ __device__ __forceinline__ float row_factor(const RowExponent &r, float scale, f
   return fmaxf(scale * 1.44269504f * gk * pow2(r.e / 2) * pow2(r.e - r.e / 2), 1e-37f);
 }
 
-// 16 consecutive query values (16-byte aligned).
+// 16 consecutive query values (16-byte aligned) as they lie in memory.
 template <int T>
-__device__ __forceinline__ void load_q16(const void *q, long long at, float *v) {
-  if constexpr (T == ROUGE_B200_T_F32) {
-    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at);
+struct RawQ {
+  static constexpr int VECS = T == ROUGE_B200_T_F32 ? 4 : 2;
+  uint4 q[VECS];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 t = p[i];
-      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
-    }
-  } else {
-    const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + at);
-    const uint4 t0 = p[0], t1 = p[1];
-    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+    for (int i = 0; i < VECS; ++i) q[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void load(const void *p, long long at) {
+    const uint4 *s = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) +
+                                                     at * (T == ROUGE_B200_T_F32 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (T == ROUGE_B200_T_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-      } else {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    for (int i = 0; i < VECS; ++i) q[i] = __ldg(s + i);
+  }
+  __device__ __forceinline__ void unpack(float *v) const {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const uint32_t u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (T == ROUGE_B200_T_F32) {
+          v[4 * i + j] = __uint_as_float(u[j]);
+        } else if constexpr (T == ROUGE_B200_T_F16) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+          v[8 * i + 2 * j] = f.x; v[8 * i + 2 * j + 1] = f.y;
+        } else {
+          v[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+          v[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        }
       }
     }
   }
+};
+template <int T>
+__device__ __forceinline__ void load_q16(const void *p, long long at, float *v) {
+  RawQ<T> r;
+  r.load(p, at);
+  r.unpack(v);
 }
 
 // Four consecutive output values (aligned to four).

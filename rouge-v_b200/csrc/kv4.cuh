@@ -28,6 +28,22 @@ inline bool valid_float_type(int type) {
   return type == ROUGE_B200_T_F32 || type == ROUGE_B200_T_F16 || type == ROUGE_B200_T_BF16;
 }
 
+// Division of n < 2^31 by a value fixed on the host (32-bit sizes): one
+// high product and a shift, with the rounded-up reciprocal
+// mul = ceil(2^(32 + shift) / d), shift = ceil(log2 d) - 1, whose error
+// n (mul d - 2^(32 + shift)) / (d 2^(32 + shift)) stays below 1 / d.
+struct Divisor {
+  unsigned d, mul, shift;
+  Divisor(unsigned v = 1) : d(v), mul(0), shift(0) {
+    if (v == 1) return;
+    while ((2u << shift) < v) ++shift;
+    mul = static_cast<unsigned>(((1ull << (32 + shift)) + v - 1) / v);
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const {
+    return d == 1 ? n : __umulhi(n, mul) >> shift;
+  }
+};
+
 // Two e4m3 codes (low byte first) as f16, exact.
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t codes) {
   uint32_t r;
