@@ -39,7 +39,16 @@ namespace rb200 {
 namespace {
 
 constexpr int kTile = 32;   // keys per tile
-constexpr int kMinTilesLog2 = 1;  // two tiles per warp before another warp joins
+// Warps at work: one per tile up to four per SM, then four tiles each, up to
+// the whole grid. A warp's plan, queries and result cost it about as much as
+// three tiles, so more of them on few tiles lose what they hide: 16384 keys of
+// 8 heads take 20 us with four tiles each, 25 with two, 36 with one; 1025
+// keys 10.6 us with one, 12.5 with two, 15.9 with four.
+__host__ __device__ __forceinline__ long long warps_at_work(long long tiles, int sms, int warps) {
+  long long w = tiles >> 2;
+  if (w < 4 * sms) w = tiles < 4 * sms ? tiles : 4 * sms;
+  return w < 1 ? 1 : (w > warps ? warps : w);
+}
 
 struct SeqInfo {
   int nq, len, q0;     // queries (at most max_q), keys, first query
@@ -183,8 +192,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     for (int i = 0; i < kWarps; ++i) total += total_slot[i];
   }
   // active warps, and this warp's range of tiles
-  long long active = total >> kMinTilesLog2;
-  active = active < 1 ? 1 : (active > a.warps ? a.warps : active);
+  const long long active = warps_at_work(total, a.sms, a.warps);
   const long long share = divide(total, active), rest = total - share * active;
   long long pos = gw * share + (gw < rest ? gw : rest);
   const long long pos_end = gw < active ? pos + share + (gw < rest ? 1 : 0) : pos;
@@ -763,14 +771,17 @@ int rows_of(int group, int max_q, int type) {
 int nt_of(int rows, int type) { return type == ROUGE_B200_T_F32 || rows == 16 ? 2 : 1; }
 
 // Warps of the grid: every SM's, fewer where even the longest sequences
-// would leave warps without kMinTiles tiles.
+// would leave warps idle.
 int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, int type) {
   const int rows = rows_of(group, max_q, type), nt = nt_of(rows, type), warps = warps_of(Dh, nt);
+  const int sms = current_sm_count(), cap = sms * ctas_of(Dh, nt) * warps;
   const double rts = std::ceil(static_cast<double>(group) * max_q / rows);
   const double tiles = max_kv < kTile ? 1.0 : std::ceil(static_cast<double>(max_kv) / kTile);
-  const int cap = current_sm_count() * ctas_of(Dh, nt);
-  const double want = std::ceil(static_cast<double>(B) * Hkv * rts * tiles / (1 << kMinTilesLog2) / warps);
-  return (want < cap ? static_cast<int>(want) : cap) * warps;
+  const double all = static_cast<double>(B) * Hkv * rts * tiles;
+  const long long w = all < 1e15 ? warps_at_work(static_cast<long long>(all), sms, cap) : cap;
+  // (few warps go one to an SM: a block for each, as far as they reach)
+  const long long ctas = w < sms ? w : (w + warps - 1) / warps < sms ? sms : (w + warps - 1) / warps;
+  return static_cast<int>(ctas) * warps;
 }
 
 size_t part_bytes(int warps, int rows, int Dh) {
@@ -879,6 +890,7 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
     return set_status(ROUGE_B200_ETOOBIG);
   a.part = static_cast<float *>(workspace);
   a.joins = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + pb);
+  a.sms = current_sm_count();
   a.row_tiles = static_cast<int>((rows + rt_rows - 1) / rt_rows);
   a.by_unit = static_cast<double>(B) * a.Hkv * a.row_tiles < a.warps ? 1 : 0;
   a.by_group = Divisor(a.group);

@@ -27,6 +27,7 @@ struct AttnArgs {
   int causal, window;
   Divisor by_group, by_page, by_heads, by_tiles;  // (by_tiles: row tiles per sequence at most)
   int warps;      // warps of the grid
+  int sms;
   float *part;    // [2 * warps][rows * (Dh + 4)]: weighted sums, then maximum and sum per row
   int4 *joins;    // units that several warps share (see attention_kv4.cu)
   int by_unit;    // joins is indexed by unit, not by warp
