@@ -625,7 +625,7 @@ int rouge_b200_transformer_block(int S, int D, int Hq, int Hkv, int Dq, int Dk, 
  * type: ROUGE_B200_T_F32, _F16 or _BF16, of x, residual and h_out, whose
  * rows need 16-byte alignment (8 bytes for the 16-bit types; 16 is faster);
  * w f32 [cols], 16-byte aligned. h_out may be x or residual itself, with
- * that array's pitch. rows == 0 does nothing. */
+ * that array's pitch. rows == 0 does nothing; rows and cols up to 2^30. */
 #define ROUGE_B200_Q_I8_ROWS 0
 #define ROUGE_B200_Q_MX_E4M3 1
 int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const void *residual,
@@ -670,17 +670,17 @@ int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void 
 /* Attention of new tokens over the cache. B sequences; sequence b has
  * kv_len[b] keys (device int32), key t of it at slot
  * page_table[b * max_pages + t / page] * page + t % page, and the queries
- * cu_q[b] .. cu_q[b + 1] (device int32 [B + 1], ascending; NULL: one query
- * per sequence), at most max_q of them. Q, O [cu_q[B]][Hq][Dh] of `type`,
+ * cu_q[b] .. cu_q[b + 1] (device int32 [B + 1], ascending from 0, the last
+ * at most the rows of Q; NULL: one query per sequence), at most max_q of them. Q, O [cu_q[B]][Hq][Dh] of `type`,
  * contiguous, 16-byte aligned. Query i of n sits at key position
  * s = kv_len[b] - n + i: causal masks t > s, window > 0 masks
  * t < s - window + 1. scale <= 0 means 1 / sqrt(Dh). Queries with no key
  * left give 0; rows of O past cu_q[B] are left as they were. Scores, softmax
  * and sums in f32; f32 queries keep f32 accuracy (the weights are rounded
  * to 11 bits for the 16-bit types). Limits: queries beyond max_q in a
- * sequence are not computed; key positions past max_pages * page, or on a
- * page number outside the cache, are taken as masked, and the next
- * rouge_b200_sync_status returns ROUGE_B200_EINVAL. The workspace
+ * sequence are not computed; key positions past max_pages * page (below
+ * 2^31 - 1023), or on a page number outside the cache, are taken as masked,
+ * and the next rouge_b200_sync_status returns ROUGE_B200_EINVAL. The workspace
  * (rouge_b200_attention_kv4_workspace bytes, 256-byte aligned, no
  * initialisation) belongs to the call until it has finished: calls that may
  * run at the same time, captured graphs among them, each need their own. */

@@ -65,9 +65,13 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) 
   s.nq = a.cu_q ? __ldg(a.cu_q + b + 1) - s.q0 : 1;
   s.len = max(0, __ldg(a.kv_len + b));
   s.p0 = s.len - s.nq;
+  if (s.len > a.max_kv) {  // (more keys than the table has pages for)
+    atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
+    s.len = a.max_kv;
+  }
   s.nq = max(0, min(s.nq, a.max_q));
   int lo = 0;
-  if (a.window > 0) lo = max(0, min(s.len, s.p0 - a.window + 1));
+  if (a.window > 0) lo = min(s.len, window_start(s.p0, a.window));
   s.lo_tile = lo / kTile;
   s.tiles = max(1, (s.len + kTile - 1) / kTile - s.lo_tile);
   s.rts = (s.nq * a.group + rows - 1) / rows;  // (rows is 8 or 16)
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     const int p0 = si.p0;
     auto q_of = [&](int r) { return static_cast<int>(a.by_group.div(r)); };  // query of a row
     const int hi_max = a.causal ? max(0, min(si.len, p0 + q_of(r1) + 1)) : si.len;
-    const int lo_min = a.window > 0 ? max(0, p0 + q_of(r0) - a.window + 1) : 0;
+    const int lo_min = a.window > 0 ? window_start(p0 + q_of(r0), a.window) : 0;
     int col_lo[S::NR][2], col_hi[S::NR][2];
     int hi_min = 0x7fffffff, lo_max = 0;
 #pragma unroll
@@ -267,10 +271,10 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         const int r = r0 + j * 8 + 2 * t + e;
         const int p = p0 + q_of(r);
         col_hi[j][e] = r < nrows ? (a.causal ? min(si.len, p + 1) : si.len) : si.len;
-        col_lo[j][e] = a.window > 0 && r < nrows ? max(0, p - a.window + 1) : 0;
+        col_lo[j][e] = a.window > 0 && r < nrows ? window_start(p, a.window) : 0;
       }
     hi_min = a.causal ? min(si.len, p0 + q_of(r0) + 1) : si.len;
-    lo_max = a.window > 0 ? max(0, p0 + q_of(r1) - a.window + 1) : 0;
+    lo_max = a.window > 0 ? window_start(p0 + q_of(r1), a.window) : 0;
     const int t_lo = max(si.lo_tile + first, lo_min / kTile);
     const int t_hi = min(si.lo_tile + last, (hi_max + kTile - 1) / kTile);
 
@@ -866,7 +870,7 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
     return set_status(ROUGE_B200_EINVAL);
   const long long max_kv = static_cast<long long>(max_pages) * cache->page;
   const long long rows = static_cast<long long>(Hq / cache->Hkv) * max_q;
-  if (max_kv > 0x7fffffffLL || rows > 0x7fffffffLL ||
+  if (max_kv > 0x7ffffc00LL || rows > 0x7ffffc00LL ||
       ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15u) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return set_status(ROUGE_B200_EUNSUPPORTED);
@@ -881,8 +885,10 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   a.B = B; a.Hq = Hq; a.group = Hq / cache->Hkv;
   a.cu_q = cu_q; a.max_q = max_q;
   a.kv_len = kv_len; a.page_table = page_table; a.max_pages = max_pages;
+  a.max_kv = static_cast<int>(max_kv);
   a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->Dh));
-  a.causal = causal; a.window = window;
+  a.causal = causal;
+  a.window = window < max_kv ? window : 0;  // (a window past the table hides nothing)
   const int rt_rows = rows_of(a.group, max_q, type);
   a.warps = grid_warps(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type);
   const size_t pb = part_bytes(a.warps, rt_rows, a.Dh);

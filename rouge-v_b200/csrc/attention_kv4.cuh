@@ -22,7 +22,7 @@ struct AttnArgs {
   int max_q;
   const int *kv_len;
   const int *page_table;
-  int max_pages;
+  int max_pages, max_kv;  // max_kv = max_pages * page
   float scale;
   int causal, window;
   Divisor by_group, by_page, by_heads, by_tiles;  // (by_tiles: row tiles per sequence at most)
@@ -41,6 +41,11 @@ bool kv4_tiles_apply(const AttnArgs &a, int type);
 int launch_attention_kv4_tiles(const AttnArgs &a, int type, cudaStream_t st);
 
 namespace {
+
+// First key a query at position p may see through the window.
+__device__ __forceinline__ int window_start(int p, int window) {
+  return p < window ? 0 : p - window + 1;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float r;

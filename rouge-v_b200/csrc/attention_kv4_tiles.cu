@@ -124,10 +124,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
   const int nq = max(0, min(n_all, a.max_q)), nrows = nq * a.group;
   const int r0 = pair * kRows;
   if (r0 >= nrows) return;
-  const int len = max(0, __ldg(a.kv_len + b)), p0 = len - n_all;
+  const int len_all = max(0, __ldg(a.kv_len + b)), p0 = len_all - n_all, len = min(len_all, a.max_kv);
+  if (len_all > a.max_kv && threadIdx.x == 0) atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
   const int r1 = min(r0 + kRows, nrows) - 1;
   const int hi_max = a.causal ? max(0, min(len, p0 + r1 / a.group + 1)) : len;
-  const int lo_min = a.window > 0 ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
+  const int lo_min = a.window > 0 ? window_start(p0 + r0 / a.group, a.window) : 0;
   const int first = lo_min / kKeys * kKeys;
   const int steps = hi_max > first ? (hi_max - first + kHalf - 1) / kHalf : 0;
   const int blocks = (steps + 1) / 2;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
     const long long at = (static_cast<long long>(qi) * a.Hq + head) * DH;
     const int pos = p0 + r / a.group;
     const int col_hi = live ? (a.causal ? min(len, pos + 1) : len) : 0x7fffffff;
-    const int col_lo = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int col_lo = live && a.window > 0 ? window_start(pos, a.window) : 0;
     float mult;
     {  // the query row, scaled to [1, 2), as f16 into the tile
       float m = 0.0f, v[16];

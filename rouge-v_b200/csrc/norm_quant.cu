@@ -451,6 +451,7 @@ extern "C" int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const 
                                             int cols, int type, void *h_out, long long ldh,
                                             int out_fmt, void *codes, void *scales, void *stream) {
   if (rows < 0 || cols <= 0 || ldx < cols) return set_status(ROUGE_B200_EINVAL);
+  if (rows > (1 << 30) || cols > (1 << 30)) return set_status(ROUGE_B200_EUNSUPPORTED);
   if (rows > 0 && (!x || !w || !codes || !scales || (residual == nullptr) != (h_out == nullptr)))
     return set_status(ROUGE_B200_EINVAL);
   if (residual && (ldr < cols || ldh < cols)) return set_status(ROUGE_B200_EINVAL);

@@ -406,6 +406,7 @@ def add_rmsnorm_quant(x, residual, w, eps, out_fmt, codes, scales, h_out=None):
     RMSNorm(h) * w: out_fmt Q_I8_ROWS (int8 [rows][cols], f32 [rows]) or Q_MX_E4M3
     (uint8 [rows][cols], uint8 [rows][cols / 32]). Rows of x, residual and h_out
     may be strided; codes and scales are contiguous."""
+    import torch
     rows, cols = x.shape
     for t in (residual, h_out):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
@@ -413,6 +414,14 @@ def add_rmsnorm_quant(x, residual, w, eps, out_fmt, codes, scales, h_out=None):
     for t in (x, residual, h_out):
         if t is not None and cols > 1 and t.stride(1) != 1:
             raise ValueError("contiguous rows expected")
+    if w.dtype != torch.float32 or w.shape != (cols,) or not w.is_contiguous():
+        raise ValueError(f"w: contiguous float32 [{cols}] expected")
+    need = ((codes, 1, rows * cols),
+            (scales, 4, rows) if out_fmt == Q_I8_ROWS else (scales, 1, rows * (cols // 32)))
+    for t, size, n in need:
+        if t.element_size() != size or t.numel() < n or not t.is_contiguous():
+            raise ValueError(f"codes, scales: {n} contiguous elements of {size} bytes expected")
+    _check_device(x, residual, w, codes, scales, h_out)
     ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else max(cols, t.stride(0))  # noqa: E731
     _check("rouge_b200_add_rmsnorm_quant", lib().rouge_b200_add_rmsnorm_quant(
         _dp(x), ld(x), _dp(residual), ld(residual), _dp(w), eps, rows, cols, _type_of(x), _dp(h_out),
@@ -425,13 +434,14 @@ class KV4Cache:
     [pages][Hkv][page][Dh / 16] (contiguous), gs_k, gs_v f32 [Hkv] or None."""
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales, gs_k=None, gs_v=None):
+        import torch
         pages, Hkv, page, half = k_codes.shape
         codes, scales = (pages, Hkv, page, half), (pages, Hkv, page, half // 8)
         for t, shape in ((k_codes, codes), (k_scales, scales), (v_codes, codes), (v_scales, scales)):
             if t.shape != shape or t.element_size() != 1 or not t.is_contiguous():
                 raise ValueError(f"contiguous bytes {shape} expected, got {tuple(t.shape)}")
         for t in (gs_k, gs_v):
-            if t is not None and (t.shape != (Hkv,) or t.element_size() != 4 or not t.is_contiguous()):
+            if t is not None and (t.shape != (Hkv,) or t.dtype != torch.float32 or not t.is_contiguous()):
                 raise ValueError(f"contiguous float32 [{Hkv}] expected")
         self.tensors = (k_codes, k_scales, v_codes, v_scales, gs_k, gs_v)
         self.pages, self.Hkv, self.page, self.Dh = pages, Hkv, page, 2 * half
@@ -455,6 +465,7 @@ def _kv4_tokens(cache, K, V, slots):
             raise ValueError(f"[{T}, {cache.Hkv}, {cache.Dh}] with contiguous tokens expected")
     if slots.shape != (T,) or slots.dtype != torch.int32 or not slots.is_contiguous():
         raise ValueError(f"slots: contiguous int32 [{T}] expected")
+    _check_device(K, V, slots, *cache.tensors)
     ld = lambda t: max(t.stride(0), cache.Hkv * cache.Dh) if T < 2 else t.stride(0)  # noqa: E731
     return (_dp(K), ld(K), _dp(V), ld(V), _type_of(K), T, _dp(slots), _stream())
 
@@ -495,6 +506,7 @@ def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scal
             raise ValueError(f"contiguous int32 {shape} expected")
     if cu_q is None and (T < B or max_q != 1):
         raise ValueError("without cu_q: one query per sequence")
+    _check_device(Q, O, kv_len, page_table, cu_q, workspace, *cache.tensors)
     ty = _type_of(Q)
     if workspace is None:
         workspace = torch.empty(attention_kv4_workspace(B, Hq, cache.Hkv, Dh, max_q,
@@ -534,6 +546,15 @@ def _type_of(t):
     return types[t.dtype]
 
 
+def _check_device(*tensors):
+    """Raises for a tensor that is not on the current CUDA device, where the launch goes."""
+    import torch
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensor on {t.device}, current device cuda:{dev}")
+
+
 class Epilogue:
     """Epilogue of gemm_i8 / gemm_e4m3 / gemm_f16: act(. + bias[n]) + residual[m][n],
     each optional. bias: f32 [N]; residual: f32, f16 or bf16 [M][N], rows
@@ -546,8 +567,8 @@ class Epilogue:
                             0 if residual is None else residual.stride(0),
                             T_F32 if residual is None else _type_of(residual), act)
 
-    def check(self, M, N):
-        """Raises unless the tensors fit an M x N output."""
+    def check(self, M, N, *others):
+        """Raises unless the tensors fit an M x N output and lie, as the others, on the current device."""
         import torch
         bias, residual = self.tensors
         if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or
@@ -555,6 +576,7 @@ class Epilogue:
             raise ValueError(f"bias: contiguous float32 [{N}] expected")
         if residual is not None and (residual.shape != (M, N) or (N > 1 and residual.stride(1) != 1)):
             raise ValueError(f"residual: [{M}, {N}] with contiguous rows expected")
+        _check_device(bias, residual, *others)
 
 
 def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None, b_cols=1,
@@ -562,7 +584,7 @@ def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N)
+        epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_i8_fused", lib().rouge_b200_gemm_i8_fused(
             M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
             C.byref(epilogue.c), _dp(C_), C_.stride(0), out_type, _stream()))
@@ -608,7 +630,7 @@ def gemm_e4m3(A, B, b_layout, C_, out_type, scale_a=None, scale_b=None, epilogue
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N)
+        epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_e4m3_fused", lib().rouge_b200_gemm_e4m3_fused(
             M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), C.byref(epilogue.c),
             _dp(C_), C_.stride(0), out_type, _stream()))
@@ -622,7 +644,7 @@ def gemm_f16(A, B, b_layout, C_, out_type, is_bf16=False, epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N)
+        epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_f16_fused", lib().rouge_b200_gemm_f16_fused(
             M, N, K, _dp(A), _dp(B), b_layout, int(is_bf16), C.byref(epilogue.c), _dp(C_),
             C_.stride(0), out_type, _stream()))

@@ -93,7 +93,8 @@ def test_epilogue(rb, cuda, kind, act, res, out):
 
 
 @pytest.mark.parametrize("layout", [0, 1])
-@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (1, 4096, 512), (16, 1040, 4096), (129, 48, 64), (2500, 4112, 128),
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (1, 4096, 512), (24, 1040, 4160), (32, 2048, 1008), (33, 2048, 1024),
+                                   (16, 8208, 640), (16, 1040, 4096), (129, 48, 64), (2500, 4112, 128),
                                    (4096, 2576, 256), (300, 8208, 144)])
 @pytest.mark.parametrize("kind", KINDS)
 def test_shapes(rb, cuda, kind, M, N, K, layout):

@@ -402,11 +402,27 @@ def test_bad_pages_are_reported_and_taken_as_masked(rb, cuda):
         assert e.value.status == rb.EINVAL
         assert torch.equal(O[1], good[1]) and O.isfinite().all()
     # a length past the table: the keys that have a page count
-    O = rb.attention_kv4(q, cache, torch.tensor([1000, 50], dtype=torch.int32, device="cuda"), table)
-    with pytest.raises(rb.RougeB200Error):
-        rb.sync_status()
-    assert torch.equal(O[1], good[1]) and (O[0] - good[0]).abs().max() < 1e-5
+    for n in (1000, 2147483647):
+        O = rb.attention_kv4(q, cache, torch.tensor([n, 50], dtype=torch.int32, device="cuda"), table)
+        with pytest.raises(rb.RougeB200Error):
+            rb.sync_status()
+        assert torch.equal(O[1], good[1]) and (O[0] - good[0]).abs().max() < 1e-5
+    # a negative one is none
+    O = rb.attention_kv4(q, cache, torch.tensor([-5, 50], dtype=torch.int32, device="cuda"), table)
+    assert torch.equal(O[1], good[1]) and (O[0] == 0).all()
+    # a window past every distance hides nothing
+    assert torch.equal(rb.attention_kv4(q, cache, lens, table, window=2147483647), good)
     rb.sync_status()
+
+
+@pytest.mark.parametrize("B", [33, 100, 700])
+def test_many_sequences(rb, cuda, B):
+    """More sequences than a warp holds at a time, empty and one-key ones among them."""
+    lens = [(7 * b) % 90 for b in range(B)]
+    nqs = [(b % 5 != 3) * (1 + (b % 7 == 0)) for b in range(B)]
+    cache = _cache(rb, sum(-(-n // 16) for n in lens) + 1, 2, 16, 64, B)
+    _check(rb, cache, "bf16", lens, nqs, 6, extra=1)
+    _check(rb, cache, "f32", lens, [1] * B, 2)
 
 
 def test_same_call_same_bits_and_shared_pages(rb, cuda):

@@ -34,7 +34,7 @@ def test_norm_invalid(rb, call, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(cols=62), dict(cols=48, fmt=1), dict(x=A + 4), dict(r=A + 8), dict(h=A + 8),
-                                dict(w=A + 8), dict(ldx=65), dict(type=1, ldx=66), dict(codes=A + 2),
+                                dict(w=A + 8), dict(ldx=65), dict(type=1, ldx=66), dict(rows=(1 << 30) + 1), dict(codes=A + 2),
                                 dict(scales=A + 1)])
 def test_norm_unsupported(rb, call, kw):
     assert call("rouge_b200_add_rmsnorm_quant", *_norm_args(**kw)) == rb.EUNSUPPORTED
@@ -161,5 +161,9 @@ def test_python_checks(rb):
         rb.Epilogue(residual=z(4, 5)).check(4, 4)
     with pytest.raises(ValueError):
         rb.attention_kv4(z(2, 4, 32), c, z(2, dtype=torch.int32), z(2, 1, dtype=torch.int32))
+    for bad in (dict(w=z(32)), dict(codes=z(3, 64, dtype=torch.int8)), dict(scales=z(4, dtype=torch.int8))):
+        a = dict(w=z(64), codes=z(4, 64, dtype=torch.int8), scales=z(4)) | bad
+        with pytest.raises(ValueError):
+            rb.add_rmsnorm_quant(z(4, 64), None, a["w"], 1e-5, 0, a["codes"], a["scales"])
     with pytest.raises(ValueError):
         rb.add_rmsnorm_quant(z(4, 64), z(4, 32), z(64), 1e-5, 0, z(4, 64, dtype=torch.int8), z(4), z(4, 64))
