@@ -416,16 +416,16 @@ def add_rmsnorm_quant(x, residual, w, eps, out_fmt, codes, scales, h_out=None):
             raise ValueError("contiguous rows expected")
     if w.dtype != torch.float32 or w.shape != (cols,) or not w.is_contiguous():
         raise ValueError(f"w: contiguous float32 [{cols}] expected")
-    need = ((codes, 1, rows * cols),
-            (scales, 4, rows) if out_fmt == Q_I8_ROWS else (scales, 1, rows * (cols // 32)))
-    for t, size, n in need:
-        if t.element_size() != size or t.numel() < n or not t.is_contiguous():
-            raise ValueError(f"codes, scales: {n} contiguous elements of {size} bytes expected")
+    size, n = (4, rows) if out_fmt == Q_I8_ROWS else (1, rows * (cols // 32))
+    if (codes.element_size() != 1 or codes.numel() < rows * cols or scales.element_size() != size or
+            scales.numel() < n or not (codes.is_contiguous() and scales.is_contiguous())):
+        raise ValueError(f"codes: {rows * cols} contiguous bytes, scales: {n} contiguous elements of {size} bytes "
+                         "expected")
     _check_device(x, residual, w, codes, scales, h_out)
     ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else max(cols, t.stride(0))  # noqa: E731
     _check("rouge_b200_add_rmsnorm_quant", lib().rouge_b200_add_rmsnorm_quant(
-        _dp(x), ld(x), _dp(residual), ld(residual), _dp(w), eps, rows, cols, _type_of(x), _dp(h_out),
-        ld(h_out), out_fmt, _dp(codes), _dp(scales), _stream()))
+        _ptr(x), ld(x), _ptr(residual), ld(residual), _ptr(w), eps, rows, cols, _type_of(x), _ptr(h_out),
+        ld(h_out), out_fmt, _ptr(codes), _ptr(scales), _stream()))
 
 
 class KV4Cache:
@@ -436,17 +436,20 @@ class KV4Cache:
     def __init__(self, k_codes, k_scales, v_codes, v_scales, gs_k=None, gs_v=None):
         import torch
         pages, Hkv, page, half = k_codes.shape
-        codes, scales = (pages, Hkv, page, half), (pages, Hkv, page, half // 8)
-        for t, shape in ((k_codes, codes), (k_scales, scales), (v_codes, codes), (v_scales, scales)):
-            if t.shape != shape or t.element_size() != 1 or not t.is_contiguous():
-                raise ValueError(f"contiguous bytes {shape} expected, got {tuple(t.shape)}")
+        codes, scales = k_codes.shape, (pages, Hkv, page, half // 8)
+        if (v_codes.shape != codes or k_scales.shape != scales or v_scales.shape != scales or
+                not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and
+                     v_scales.is_contiguous()) or k_codes.element_size() != 1 or k_scales.element_size() != 1 or
+                v_codes.element_size() != 1 or v_scales.element_size() != 1):
+            raise ValueError(f"codes: contiguous bytes {tuple(codes)}, scales: {scales} expected")
         for t in (gs_k, gs_v):
             if t is not None and (t.shape != (Hkv,) or t.dtype != torch.float32 or not t.is_contiguous()):
                 raise ValueError(f"contiguous float32 [{Hkv}] expected")
         self.tensors = (k_codes, k_scales, v_codes, v_scales, gs_k, gs_v)
         self.pages, self.Hkv, self.page, self.Dh = pages, Hkv, page, 2 * half
-        self.c = _KV4C(*(None if t is None else t.data_ptr() for t in self.tensors), pages, page, Hkv,
-                       2 * half)
+        self.c = _KV4C(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                       _ptr(gs_k), _ptr(gs_v), pages, page, Hkv, 2 * half)
+        self.ref = C.byref(self.c)
 
     @classmethod
     def empty(cls, pages, Hkv, page, Dh, gs_k=None, gs_v=None, device="cuda"):
@@ -467,20 +470,20 @@ def _kv4_tokens(cache, K, V, slots):
         raise ValueError(f"slots: contiguous int32 [{T}] expected")
     _check_device(K, V, slots, *cache.tensors)
     ld = lambda t: max(t.stride(0), cache.Hkv * cache.Dh) if T < 2 else t.stride(0)  # noqa: E731
-    return (_dp(K), ld(K), _dp(V), ld(V), _type_of(K), T, _dp(slots), _stream())
+    return (K.data_ptr(), ld(K), V.data_ptr(), ld(V), _type_of(K), T, slots.data_ptr(), _stream())
 
 
 def kv4_write(cache, K, V, slots):
     """K, V [T][Hkv][Dh] (f32, f16 or bf16; tokens may be strided) into the
     slots [T] (int32; negative: skipped) of a KV4Cache."""
     _check("rouge_b200_kv4_write",
-           lib().rouge_b200_kv4_write(C.byref(cache.c), *_kv4_tokens(cache, K, V, slots)))
+           lib().rouge_b200_kv4_write(cache.ref, *_kv4_tokens(cache, K, V, slots)))
 
 
 def kv4_read(cache, slots, K, V):
     """The values of slots [T] into K, V [T][Hkv][Dh]."""
     _check("rouge_b200_kv4_read",
-           lib().rouge_b200_kv4_read(C.byref(cache.c), *_kv4_tokens(cache, K, V, slots)))
+           lib().rouge_b200_kv4_read(cache.ref, *_kv4_tokens(cache, K, V, slots)))
 
 
 def attention_kv4_workspace(B, Hq, Hkv, Dh, max_q, max_kv, type):
@@ -501,11 +504,15 @@ def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scal
         raise ValueError("Q, O: contiguous, of one shape and type")
     if Dh != cache.Dh:
         raise ValueError(f"head size {Dh}, and {cache.Dh} in the cache")
-    for t, shape in ((kv_len, (B,)), (page_table, (B, max_pages)), (cu_q, (B + 1,))):
-        if t is not None and (t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous()):
-            raise ValueError(f"contiguous int32 {shape} expected")
-    if cu_q is None and (T < B or max_q != 1):
-        raise ValueError("without cu_q: one query per sequence")
+    i32 = torch.int32
+    if (kv_len.dtype != i32 or kv_len.shape != (B,) or page_table.dtype != i32 or
+            not (kv_len.is_contiguous() and page_table.is_contiguous())):
+        raise ValueError(f"contiguous int32 kv_len [{B}] and page_table [{B}, {max_pages}] expected")
+    if cu_q is None:
+        if T < B or max_q != 1:
+            raise ValueError("without cu_q: one query per sequence")
+    elif cu_q.dtype != i32 or cu_q.shape != (B + 1,) or not cu_q.is_contiguous():
+        raise ValueError(f"cu_q: contiguous int32 [{B + 1}] expected")
     _check_device(Q, O, kv_len, page_table, cu_q, workspace, *cache.tensors)
     ty = _type_of(Q)
     if workspace is None:
@@ -513,8 +520,8 @@ def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scal
                                                         max_pages * cache.page, ty),
                                 dtype=torch.uint8, device=Q.device)
     _check("rouge_b200_attention_kv4", lib().rouge_b200_attention_kv4(
-        C.byref(cache.c), _dp(Q), ty, B, Hq, _dp(cu_q), max_q, _dp(kv_len), _dp(page_table), max_pages,
-        _dp(O), scale, causal, window, _dp(workspace), workspace.numel(), _stream()))
+        cache.ref, Q.data_ptr(), ty, B, Hq, _ptr(cu_q), max_q, kv_len.data_ptr(), page_table.data_ptr(),
+        max_pages, O.data_ptr(), scale, causal, window, workspace.data_ptr(), workspace.numel(), _stream()))
     return O
 
 
@@ -537,13 +544,22 @@ T_F32, T_F16, T_BF16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 
+_types = {}
+
+
 def _type_of(t):
     """ROUGE_B200_T_* of a floating tensor."""
-    import torch
-    types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
-    if t.dtype not in types:
+    if not _types:
+        import torch
+        _types.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16})
+    ty = _types.get(t.dtype)
+    if ty is None:
         raise TypeError(f"float32, float16 or bfloat16 tensor expected, got {t.dtype}")
-    return types[t.dtype]
+    return ty
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _check_device(*tensors):
@@ -566,6 +582,7 @@ class Epilogue:
                             None if residual is None else residual.data_ptr(),
                             0 if residual is None else residual.stride(0),
                             T_F32 if residual is None else _type_of(residual), act)
+        self.ref = C.byref(self.c)
 
     def check(self, M, N, *others):
         """Raises unless the tensors fit an M x N output and lie, as the others, on the current device."""
@@ -586,8 +603,8 @@ def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None
     if epilogue is not None:
         epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_i8_fused", lib().rouge_b200_gemm_i8_fused(
-            M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
-            C.byref(epilogue.c), _dp(C_), C_.stride(0), out_type, _stream()))
+            M, N, K, _ptr(A), _ptr(B), b_layout, _ptr(scales_a), a_rows, _ptr(scales_b), b_cols,
+            epilogue.ref, _ptr(C_), C_.stride(0), out_type, _stream()))
         return
     _check("rouge_b200_gemm_i8", lib().rouge_b200_gemm_i8(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
@@ -632,8 +649,8 @@ def gemm_e4m3(A, B, b_layout, C_, out_type, scale_a=None, scale_b=None, epilogue
     if epilogue is not None:
         epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_e4m3_fused", lib().rouge_b200_gemm_e4m3_fused(
-            M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), C.byref(epilogue.c),
-            _dp(C_), C_.stride(0), out_type, _stream()))
+            M, N, K, _ptr(A), _ptr(B), b_layout, _ptr(scale_a), _ptr(scale_b), epilogue.ref,
+            _ptr(C_), C_.stride(0), out_type, _stream()))
         return
     _check("rouge_b200_gemm_e4m3", lib().rouge_b200_gemm_e4m3(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), _dp(C_), C_.stride(0),
@@ -646,7 +663,7 @@ def gemm_f16(A, B, b_layout, C_, out_type, is_bf16=False, epilogue=None):
     if epilogue is not None:
         epilogue.check(M, N, A, B, C_)
         _check("rouge_b200_gemm_f16_fused", lib().rouge_b200_gemm_f16_fused(
-            M, N, K, _dp(A), _dp(B), b_layout, int(is_bf16), C.byref(epilogue.c), _dp(C_),
+            M, N, K, _ptr(A), _ptr(B), b_layout, int(is_bf16), epilogue.ref, _ptr(C_),
             C_.stride(0), out_type, _stream()))
         return
     _check("rouge_b200_gemm_f16", lib().rouge_b200_gemm_f16(
