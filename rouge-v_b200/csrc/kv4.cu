@@ -4,8 +4,11 @@
 // registers, so the block's maximum needs no shuffle, and 8 bytes of codes
 // plus one scale byte out (or the reverse). Neighbouring threads hold
 // neighbouring blocks, so a warp reads whole lines of K or V and writes
-// whole sectors of the page. Memory-bound: 2 or 4 bytes in and 0.5625 bytes
-// out per value.
+// whole sectors of the page. The floor is memory: 2 or 4 bytes in and 0.5625
+// bytes out per value. 32768 bf16 tokens of 8 x 128: 39.4 us to write (66 % of
+// the copy rate; 58 % of the integer pipe, about 200 instructions per thread),
+// 41.0 to read (64 %; the warps wait for their loads). Two blocks per thread
+// in flight gained nothing in either.
 #include <cuda_runtime.h>
 
 #include <cstdint>
