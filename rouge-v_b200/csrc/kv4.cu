@@ -5,10 +5,9 @@
 // plus one scale byte out (or the reverse). Neighbouring threads hold
 // neighbouring blocks, so a warp reads whole lines of K or V and writes
 // whole sectors of the page. The floor is memory: 2 or 4 bytes in and 0.5625
-// bytes out per value. 32768 bf16 tokens of 8 x 128: 39.4 us to write (66 % of
+// bytes out per value. 32768 bf16 tokens of 8 x 128: 39.2 us to write (67 % of
 // the copy rate; 58 % of the integer pipe, about 200 instructions per thread),
-// 41.0 to read (64 %; the warps wait for their loads). Two blocks per thread
-// in flight gained nothing in either.
+// 30.8 to read (85 %). Two blocks per thread in flight gained nothing in either.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -31,25 +30,53 @@ struct KvArgs {
   long long ld[2];
   int page, Hkv, nblk;  // nblk = Dh / 16
   Divisor by_nblk, by_heads, by_page;
+  int wide[2];  // source (or destination) and pitch are multiples of 32 bytes
   int total_slots;
   unsigned items;       // tokens * Hkv * nblk of this launch
   const int *slots;
   int *err;
 };
 
+// 32 bytes in one access (a thread's block is 32 or 64 bytes: two accesses of
+// 16 would touch each of the warp's lines twice: 41.0 us instead of 30.8 to read
+// 32768 bf16 tokens of 8 x 128; writing them gains 0.2).
+__device__ __forceinline__ void ld32(const void *p, bool wide, uint32_t (&u)[8]) {
+  if (wide) {
+    asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+        : "l"(p));
+    return;
+  }
+  const uint4 *q = static_cast<const uint4 *>(p);
+  const uint4 t0 = __ldg(q), t1 = __ldg(q + 1);
+  u[0] = t0.x; u[1] = t0.y; u[2] = t0.z; u[3] = t0.w;
+  u[4] = t1.x; u[5] = t1.y; u[6] = t1.z; u[7] = t1.w;
+}
+
+__device__ __forceinline__ void st32(void *p, bool wide, const uint32_t (&u)[8]) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]),
+                 "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
+    return;
+  }
+  uint4 *q = static_cast<uint4 *>(p);
+  q[0] = make_uint4(u[0], u[1], u[2], u[3]);
+  q[1] = make_uint4(u[4], u[5], u[6], u[7]);
+}
+
 template <int T>
-__device__ __forceinline__ void load16(const void *p, long long at, float (&v)[16]) {
+__device__ __forceinline__ void load16(const void *p, long long at, bool wide, float (&v)[16]) {
+  uint32_t u[8];
   if constexpr (T == ROUGE_B200_T_F32) {
-    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 t = __ldg(q + i);
-      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+    for (int k = 0; k < 2; ++k) {
+      ld32(static_cast<const float *>(p) + at + 8 * k, wide, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[8 * k + i] = __uint_as_float(u[i]);
     }
   } else {
-    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
-    const uint4 t0 = __ldg(q), t1 = __ldg(q + 1);
-    const uint32_t u[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+    ld32(static_cast<const uint16_t *>(p) + at, wide, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (T == ROUGE_B200_T_F16) {
@@ -64,19 +91,20 @@ __device__ __forceinline__ void load16(const void *p, long long at, float (&v)[1
 }
 
 template <int T>
-__device__ __forceinline__ void store16(void *p, long long at, const float (&v)[16]) {
+__device__ __forceinline__ void store16(void *p, long long at, bool wide, const float (&v)[16]) {
+  uint32_t u[8];
   if constexpr (T == ROUGE_B200_T_F32) {
-    float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[8 * k + i]);
+      st32(static_cast<float *>(p) + at + 8 * k, wide, u);
+    }
   } else {
-    uint32_t u[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       u[i] = T == ROUGE_B200_T_F16 ? f16x2_rn(v[2 * i], v[2 * i + 1]) : bf16x2_rn(v[2 * i], v[2 * i + 1]);
-    uint4 *q = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at);
-    q[0] = make_uint4(u[0], u[1], u[2], u[3]);
-    q[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    st32(static_cast<uint16_t *>(p) + at, wide, u);
   }
 }
 
@@ -128,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
     size_t at;
     if (!locate(a, i, head, el, which, at)) continue;
     float v[16];
-    load16<T>(a.src[which], el, v);
+    load16<T>(a.src[which], el, a.wide[which], v);
     const float g = a.gs[which] ? __ldg(a.gs[which] + head) : 1.0f;
     float m = 0.0f;
 #pragma unroll
@@ -185,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const KvArgs a) {
         v[8 * k + 2 * j + 1] = __fmul_rn(__fmul_rn(f.y, s), g);
       }
     }
-    store16<T>(a.dst[which], el, v);
+    store16<T>(a.dst[which], el, a.wide[which], v);
   }
 }
 
@@ -205,6 +233,8 @@ int prepare(const RougeB200KV4 *c, const void *K, long long ldk, const void *V, 
   a.scales[0] = c->k_scales; a.scales[1] = c->v_scales;
   a.gs[0] = c->gs_k; a.gs[1] = c->gs_v;
   a.ld[0] = ldk; a.ld[1] = ldv;
+  a.wide[0] = (reinterpret_cast<uintptr_t>(K) & 31u) == 0 && (ldk * es) % 32 == 0;
+  a.wide[1] = (reinterpret_cast<uintptr_t>(V) & 31u) == 0 && (ldv * es) % 32 == 0;
   a.page = c->page;
   a.Hkv = c->Hkv;
   a.nblk = c->Dh / 16;

@@ -190,6 +190,38 @@ def test_write_and_read(rb, cuda, t, T, Hkv, Dh, page, gs):
         assert (back[~keep] == 9).all()
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shift,pad", [(0, 0), (16, 0), (0, 16), (16, 16), (32, 32)])
+def test_write_and_read_on_16_byte_boundaries(rb, cuda, t, shift, pad):
+    """Tokens at any multiple of 16 bytes, K's and V's independently: the codes and values of aligned ones,
+    and nothing written between the rows."""
+    import torch
+    T, Hkv, Dh, page = 37, 3, 48, 16
+    dt, es = _dt(t), torch.empty((), dtype=_dt(t)).element_size()
+    x = torch.randn(T, Hkv, Dh, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(dt)
+    slots = torch.arange(T, dtype=torch.int32, device="cuda")
+
+    def view(fill):
+        buf = torch.full(((shift + T * (Hkv * Dh * es + pad)) // es,), fill, dtype=dt, device="cuda")
+        return buf, buf[shift // es:].as_strided((T, Hkv, Dh), (Hkv * Dh + pad // es, Dh, 1), shift // es)
+
+    aligned, moved = (rb.KV4Cache.empty(3, Hkv, page, Dh) for _ in range(2))
+    rb.kv4_write(aligned, x, x, slots)
+    _, y = view(0)
+    y.copy_(x)
+    rb.kv4_write(moved, y, x, slots)
+    for a, b in zip(aligned.tensors[:4], moved.tensors[:4]):
+        assert torch.equal(a, b)
+    want, other = torch.empty_like(x), torch.empty_like(x)
+    rb.kv4_read(aligned, slots, want, other)
+    buf, z = view(7)
+    rb.kv4_read(aligned, slots, other, z)
+    rb.sync_status()
+    assert torch.equal(z, want) and torch.equal(other, want)
+    z.fill_(7)
+    assert (buf == 7).all()
+
+
 def test_write_ties_and_specials(rb, cuda):
     """Every border between two codes, saturation, signed zeros, NaN and infinities, subnormal and huge scales."""
     import torch
