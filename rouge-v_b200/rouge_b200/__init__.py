@@ -515,6 +515,8 @@ def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scal
         raise ValueError(f"cu_q: contiguous int32 [{B + 1}] expected")
     _check_device(Q, O, kv_len, page_table, cu_q, workspace, *cache.tensors)
     ty = _type_of(Q)
+    if T == 0:  # (an empty tensor has no address)
+        return O
     if workspace is None:
         workspace = torch.empty(attention_kv4_workspace(B, Hq, cache.Hkv, Dh, max_q,
                                                         max_pages * cache.page, ty),

@@ -247,6 +247,16 @@ def test_write_ties_and_specials(rb, cuda):
         assert (got[0][5] == 0).all() and (got[1][5] == 0).all()
 
 
+def test_attention_without_queries(rb, cuda):
+    import torch
+    cache = rb.KV4Cache.empty(2, 1, 16, 64)
+    z = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.empty(0, 4, 64, device="cuda")
+    o = rb.attention_kv4(q, cache, z[:2], torch.zeros(2, 1, dtype=torch.int32, device="cuda"), cu_q=z)
+    rb.sync_status()
+    assert o.shape == q.shape
+
+
 def test_bad_slots_are_reported(rb, cuda):
     import torch
     cache = rb.KV4Cache.empty(2, 2, 16, 32)
