@@ -156,9 +156,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
     tmem_alloc(tmem_slot, C::COLS);
     tmem_relinquish();
   }
+  // whether the table names a page outside the cache among those with keys
+  // some row sees (their keys are masked; an error, so the masks are only
+  // worked out where there is one)
+  const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
+  auto page_ok = [&](int pi) {
+    const int id = __ldg(table + pi);
+    return id >= 0 && id < a.pages;
+  };
+  int bad = 0;
+  if (steps > 0)  // (hi_max <= max_kv: every such page is in the table)
+    for (int pi = lo_min / a.page + threadIdx.x; pi <= (hi_max - 1) / a.page; pi += kThreads)
+      bad |= !page_ok(pi);
   tc_fence_before_sync();
-  __syncthreads();
+  const bool holes = __syncthreads_or(bad);
   tc_fence_after_sync();
+  if (holes && threadIdx.x == 0) atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
   const uint32_t tmem = *tmem_slot;
   auto fail = [&]() {
     *abort = 1;
@@ -228,6 +241,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
             const int key = key0 + 32 * c + k;
             if (key < col_lo || key >= col_hi) x[c][k] = 0xFF800000u;  // -inf
           }
+      }
+      if (holes) {  // (a page holds whole groups of 16 keys)
+        const int key = key0 + 16 * (lane & 3);
+        const unsigned there =
+            __ballot_sync(0xffffffffu, key >= hi_max || key + 16 <= lo_min || page_ok(key / a.page));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!((there >> (2 * c + k / 16)) & 1u)) x[c][k] = 0xFF800000u;
       }
       float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -310,7 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
   } else if (warp < 12) {
     // ------------------------------------------------------------ K and V rows
     const int kr = threadIdx.x - 256;
-    const int *table = a.page_table + static_cast<size_t>(b) * a.max_pages;
     KeyRow<DH> k, v;
     auto fetch = [&](int j) {
       k.zero();
@@ -318,11 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
       const int key = first + j * kKeys + kr;
       if (j >= blocks || key >= hi_max || key < lo_min) return;  // (a key of no row: zeros)
       const int pi = key / a.page;
-      const int id = pi < a.max_pages ? __ldg(table + pi) : -1;
-      if (id < 0 || id >= a.pages) {
-        atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
-        return;
-      }
+      const int id = __ldg(table + pi);
+      if (id < 0 || id >= a.pages) return;  // (masked)
       const size_t row = (static_cast<size_t>(id) * a.Hkv + hk) * a.page + (key - pi * a.page);
       k.load(a.k_codes, a.k_scales, row);
       v.load(a.v_codes, a.v_scales, row);

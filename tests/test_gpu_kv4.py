@@ -562,3 +562,60 @@ def test_decoder_step_together(rb, cuda):
         wo_ = (aq.double() @ o_q.double().T) * asc.double()[:, None] * o_s.double() + h.double()
         assert ((out.double() - wo_).abs() <= wo_.abs() * 2.0 ** -8 + 2.0 ** -20).all()
         res = out
+
+
+def _sequence_reference(cache, q, n, row, window, hidden, tiny_step):
+    """O and the tolerance's parts of one causal sequence in 64 bits, without its keys t where hidden[t]."""
+    import torch
+    kc, ks, vc, vs, gk, gv = cache.tensors
+    one = torch.ones(cache.Hkv, device="cuda")
+    nq, G = q.shape[0], q.shape[1] // cache.Hkv
+    t = torch.arange(n, device="cuda")
+    pg, off = row.long().clamp(0, cache.pages - 1)[t // cache.page], t % cache.page
+    K = _decode(kc, ks, gk if gk is not None else one)[pg, :, off].repeat_interleave(G, 1)
+    V = _decode(vc, vs, gv if gv is not None else one)[pg, :, off].repeat_interleave(G, 1)
+    p = n - nq + torch.arange(nq, device="cuda")[:, None]
+    ok = (t <= p) & ~hidden & ((t > p - window) if window else True)
+    scale = cache.Dh ** -0.5
+    z = torch.einsum("ihd,thd->hit", q.double(), K) * scale
+    za = torch.einsum("ihd,thd->hit", q.double().abs(), K.abs()) * scale
+    w = torch.softmax(z.masked_fill(~ok, -math.inf), -1).nan_to_num(0)  # (a row without keys)
+    ds = (za.masked_fill(~ok, 0).amax(-1) * (cache.Dh / 16 + 6) * 2.0 ** -23).T[..., None]
+    return (torch.einsum("hit,thd->ihd", w, V), torch.einsum("hit,thd->ihd", w, V.abs()), ds,
+            tiny_step * torch.einsum("it,thd->ihd", ok.double(), V.abs()))
+
+
+def _close(O, want, spread, ds, tiny, t, n):
+    w = 2.0 ** -21 + (2.0 ** -21 if t == "f32" else 2.0 ** -11)
+    tol = (2 * ds + w + (max(n, 16) / 16 + 64) * 2.0 ** -23) * spread + tiny
+    tol = tol + _half_step(want.abs() + tol, O.dtype)
+    d = (O.double() - want).abs()
+    assert (d <= tol).all(), ((d / tol.clamp(min=1e-300)).nan_to_num(math.inf).max().item(), d.max().item())
+
+
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("t,nq,Hq,Dh", [("f32", 1, 4, 64), ("bf16", 1, 4, 128), ("f16", 20, 8, 80),
+                                        ("bf16", 500, 16, 128), ("f16", 700, 16, 64)])
+def test_keys_on_bad_pages_have_no_weight(rb, cuda, t, nq, Hq, Dh, window):
+    """Scores far below zero: a key taken in with a score of zero would outweigh all others."""
+    import torch
+    Hkv, page, n = 4, 16, 730
+    g = torch.Generator("cuda").manual_seed(nq + Dh)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    cache = rb.KV4Cache.empty(46, Hkv, page, Dh)
+    x = rn(1, Hkv, Dh)
+    rb.kv4_write(cache, -x + 0.3 * rn(n, Hkv, Dh), rn(n, Hkv, Dh), torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = (x.repeat_interleave(Hq // Hkv, 1) + 0.2 * rn(nq, Hq, Dh)).to(_dt(t))
+    table = torch.arange(46, dtype=torch.int32, device="cuda")[None].clone()
+    hidden = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for i, bad in ((0, -1), (14, 46), (15, 1 << 30), (41, -1 << 31), (45, 46)):
+        table[0, i] = bad
+        hidden[i * page:(i + 1) * page] = True
+    cu = torch.tensor([0, nq], dtype=torch.int32, device="cuda")
+    O = rb.attention_kv4(q, cache, torch.tensor([n], dtype=torch.int32, device="cuda"), table, cu_q=cu, max_q=nq,
+                         window=window)
+    with pytest.raises(rb.RougeB200Error) as e:
+        rb.sync_status()
+    assert e.value.status == rb.EINVAL
+    tiny = 2.0 ** -32 if nq >= 500 else 2.0 ** -40
+    _close(O, *_sequence_reference(cache, q, n, table[0], window, hidden, tiny), t, n)
