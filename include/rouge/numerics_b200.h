@@ -676,8 +676,10 @@ int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void 
  * s = kv_len[b] - n + i: causal masks t > s, window > 0 masks
  * t < s - window + 1. scale <= 0 means 1 / sqrt(Dh). Queries with no key
  * left give 0; rows of O past cu_q[B] are left as they were. Scores, softmax
- * and sums in f32; f32 queries keep f32 accuracy (the weights are rounded
- * to 11 bits for the 16-bit types). Limits: queries beyond max_q in a
+ * and sums in f32. f32 queries are held to 2^-23 of each value (or 2^-50 of
+ * their row's largest), f16 ones exactly, bf16 ones exactly (or to 2^-40 of
+ * the largest); softmax weights to 2^-23 for f32 and 2^-11 for the 16-bit
+ * types (or, of the largest weight, 2^-40, in long prompt chunks 2^-32). Limits: queries beyond max_q in a
  * sequence are not computed; key positions past max_pages * page (below
  * 2^31 - 1023), or on a page number outside the cache, are taken as masked,
  * and the next rouge_b200_sync_status returns ROUGE_B200_EINVAL. The workspace

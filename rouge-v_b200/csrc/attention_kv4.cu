@@ -21,10 +21,11 @@
 // takes a run of Dh / 4 values of its key rows, and of Dh / 8 columns of its
 // value rows, read with 8- or 16-byte loads.
 //
-// code * scale has 2 + 4 significand bits: exact in f16, as are 16-bit
-// queries (scaled to [1, 2) by a power of two per row). f32 queries are split
-// into two f16 parts held in two row tiles, whose scores add up; the weights
-// are split the same way. Accumulation is f32.
+// code * scale has 2 + 4 significand bits: exact in f16. Queries are scaled by
+// a power of two per row to the top of f16's range (row_exponent says what of
+// them is held). f32 queries are split into two f16 parts held in two row
+// tiles, whose scores are added; the weights, times 2^15, are split the same
+// way. Accumulation is f32.
 //
 // What bounds it is instruction issue: 64 sequences of up to 8192 keys, Hq 64,
 // Hkv 8, Dh 128 take 98.5 us, 59 % of the copy rate, with 63 % of the issue
@@ -141,7 +142,7 @@ constexpr int warps_of(int Dh, int nt) { return Dh > 128 || nt == 1 ? 8 : 12; }
 constexpr int ctas_of(int Dh, int nt) { return Dh > 128 || nt == 2 ? 1 : 2; }
 
 // DT: Dh rounded up to 64, 128 or 256. NT: tiles of 8 mma columns. f32
-// queries: columns 8.. hold the low parts of rows 0.., so 4 * NT rows.
+// queries: columns 8.. hold the low parts (times 2^11) of rows 0.., so 4 * NT rows.
 template <int DT, int NT, int T>
 struct Shape {
   static constexpr bool SPLIT = T == ROUGE_B200_T_F32;
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
     int ahead = t_lo;
     for (; ahead < t_hi && ahead < t_lo + S::STAGES - 1; ++ahead) issue(ahead);
 
-    // ---- queries as B fragments, scaled to [1, 2) per row
+    // ---- queries as B fragments, scaled per row
     uint32_t qf[NT][kSteps][2];
     float mult[S::NR][2];
     {
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
         for (int k = 0; k < DT / 4; ++k) m = fmaxf(m, fabsf(v[k]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const RowExponent re = row_exponent(m);
+        const RowExponent re = row_exponent<T>(m);
 #pragma unroll
         for (int k = 0; k < DT / 4; ++k) v[k] = v[k] * re.down * re.down2;
 #pragma unroll
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
             qf[j][s][p] = hi;
             if constexpr (S::SPLIT) {
               const float2 b2 = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-              qf[S::NR + j][s][p] = f16x2_rn(x0 - b2.x, x1 - b2.y);
+              qf[S::NR + j][s][p] = f16x2_rn((x0 - b2.x) * kSplitScale, (x1 - b2.y) * kSplitScale);
             }
           }
         const float mine = row_factor(re, a.scale, gk);
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(warps_of(DT, NT) * 32, ctas_of(DT, NT))
 #pragma unroll
           for (int j = 0; j < S::NR; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[kb][j][e] += sc[kb][S::NR + j][e];
+            for (int e = 0; e < 4; ++e)
+              sc[kb][j][e] = __fmaf_rn(sc[kb][S::NR + j][e], 1.0f / kSplitScale, sc[kb][j][e]);
       }
       if (masked) {
 #pragma unroll

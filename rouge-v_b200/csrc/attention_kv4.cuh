@@ -56,18 +56,27 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// The power-of-two exponent of a row of queries whose largest magnitude is m,
-// and factors that take it out: the row is scaled to [1, 2) before it is
-// rounded to f16, the scores by 2^e afterwards.
+// The power of two that takes a row of queries, whose largest magnitude is m,
+// to the top of f16's range before it is rounded, 2^(kTop - 1) <= largest <
+// 2^kTop, and its factors; the scores are multiplied by 2^e afterwards. 16-bit
+// rows have kTop = 16: f16 values are held exactly, bf16 ones down to 2^-32 of
+// the row's largest, below which they are off by at most 2^-40 of it. f32 rows
+// have kTop = 15 (their high part is rounded, maybe up) and two parts, high and
+// the rest times 2^11, which hold a value to 2^-23 of itself down to 2^-27 of
+// the row's largest, and to 2^-50 of the largest below that.
 struct RowExponent {
   int e;
   float down, down2;
 };
+constexpr float kSplitScale = 2048.0f;
+template <int T>
 __device__ __forceinline__ RowExponent row_exponent(float m) {
+  constexpr int kTop = T == ROUGE_B200_T_F32 ? 15 : 16;
   RowExponent r;
   r.e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
-  if (r.e == 128) r.e = 0;          // (infinity or NaN)
+  if (r.e == 128) r.e = kTop - 1;   // (infinity or NaN: as it is)
   r.e = r.e < -100 ? -100 : r.e;    // (tiny rows stay tiny)
+  r.e -= kTop - 1;
   r.down = pow2(-(r.e / 2));
   r.down2 = pow2(-(r.e - r.e / 2));
   return r;

@@ -25,8 +25,8 @@
 // the MMAs would be 1330 by the rates of single ones (51.7 cycles at N = 64,
 // 64 at N = 128) and the 16384 exponentials 1024 on 16 lanes a cycle; the rest
 // are the groups' starts. 2 x 512 queries of 32 heads over up to 4096 keys: 92
-// us, 557 TFLOP/s. code * scale is exact in f16, as are 16-bit
-// queries scaled by a power of two per row; weights are rounded to f16.
+// us, 557 TFLOP/s. code * scale is exact in f16; 16-bit queries are
+// held as row_exponent says; weights are rounded to f16.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
     const int col_hi = live ? (a.causal ? min(len, pos + 1) : len) : 0x7fffffff;
     const int col_lo = live && a.window > 0 ? window_start(pos, a.window) : 0;
     float mult;
-    {  // the query row, scaled to [1, 2), as f16 into the tile
+    {  // the query row, scaled by a power of two, as f16 into the tile
       float m = 0.0f, v[16];
       if (live) {
 #pragma unroll
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
           for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
         }
       }
-      const RowExponent re = row_exponent(m);
+      const RowExponent re = row_exponent<T>(m);
       mult = row_factor(re, a.scale, a.gs_k ? __ldg(a.gs_k + hk) : 1.0f);
 #pragma unroll
       for (int k = 0; k < DH / 16; ++k) {

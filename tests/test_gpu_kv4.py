@@ -619,3 +619,26 @@ def test_keys_on_bad_pages_have_no_weight(rb, cuda, t, nq, Hq, Dh, window):
     assert e.value.status == rb.EINVAL
     tiny = 2.0 ** -32 if nq >= 500 else 2.0 ** -40
     _close(O, *_sequence_reference(cache, q, n, table[0], window, hidden, tiny), t, n)
+
+
+@pytest.mark.parametrize("t,up", [("f32", 10), ("f32", 14), ("f32", 20), ("bf16", 14), ("bf16", 24), ("f16", 14)])
+@pytest.mark.parametrize("nq,Hq,Dh", [(1, 4, 64), (1, 32, 128), (9, 4, 256), (400, 16, 128)])
+def test_query_channels_far_above_the_others(rb, cuda, t, up, nq, Hq, Dh):
+    """Two channels 2^up above the rest meet zero codes: the scores are those of the small channels, whose values
+    are held to 2^-23 of their own size (16-bit queries exactly), not of the largest one's."""
+    import torch
+    n = 410
+    cache = _cache(rb, 26, 4, 16, Dh, up)
+    kc = cache.tensors[0]
+    kc[..., 2] &= 0xF0       # channel 4
+    kc[..., Dh // 2 - 1] &= 0x0F  # channel Dh - 1
+    g = torch.Generator("cuda").manual_seed(nq + Dh)
+    q = torch.randn(nq, Hq, Dh, generator=g, device="cuda")
+    q[..., 4], q[..., Dh - 1] = 1.37 * 2.0 ** up, -1.9 * 2.0 ** up
+    q = q.to(_dt(t))
+    table = torch.randperm(26, generator=g, device="cuda").int()[None]
+    cu = torch.tensor([0, nq], dtype=torch.int32, device="cuda")
+    O = rb.attention_kv4(q, cache, torch.tensor([n], dtype=torch.int32, device="cuda"), table, cu_q=cu, max_q=nq)
+    rb.sync_status()
+    hidden = torch.zeros(n, dtype=torch.bool, device="cuda")
+    _close(O, *_sequence_reference(cache, q, n, table[0], 0, hidden, 2.0 ** -32 if nq == 400 else 2.0 ** -40), t, n)
