@@ -66,15 +66,15 @@ struct SeqInfo {
 // Work of sequence b for row tiles of `rows` rows.
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) {
   SeqInfo s;
-  s.q0 = a.cu_q ? __ldg(a.cu_q + b) : b;
-  s.nq = a.cu_q ? __ldg(a.cu_q + b + 1) - s.q0 : 1;
+  const SeqQueries q = seq_queries(a, b, a.err);
+  s.q0 = q.q0;
+  s.nq = q.n;
   s.len = max(0, __ldg(a.kv_len + b));
-  s.p0 = s.len - s.nq;
+  s.p0 = s.len - q.all;
   if (s.len > a.max_kv) {  // (more keys than the table has pages for)
     atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
     s.len = a.max_kv;
   }
-  s.nq = max(0, min(s.nq, a.max_q));
   int lo = 0;
   if (a.window > 0) lo = min(s.len, window_start(s.p0, a.window));
   s.lo_tile = lo / kTile;
@@ -713,9 +713,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
     rt = a.by_heads.div(u.y);
     hk = u.y - rt * a.Hkv;
   }
-  const int q0 = a.cu_q ? a.cu_q[b] : b;
-  int nq = a.cu_q ? a.cu_q[b + 1] - q0 : 1;
-  nq = max(0, min(nq, a.max_q));
+  const SeqQueries sq = seq_queries(a, b, nullptr);
+  const int q0 = sq.q0, nq = sq.n;
   const int share = rows / gridDim.y, first = blockIdx.y * share;
   const int live = min(share, nq * a.group - rt * rows - first);  // this block's rows
   if (live <= 0 || u.w < 2) return;

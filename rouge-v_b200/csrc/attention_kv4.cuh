@@ -42,6 +42,25 @@ int launch_attention_kv4_tiles(const AttnArgs &a, int type, cudaStream_t st);
 
 namespace {
 
+// The queries of sequence b: first row, their number (all of them, and those
+// that are computed). More than max_q, or offsets that fall or start below
+// zero, are reported to `err` where it is given.
+struct SeqQueries {
+  int q0, all, n;
+};
+__device__ __forceinline__ SeqQueries seq_queries(const AttnArgs &a, int b, int *err) {
+  SeqQueries q{b, 1, 1};
+  if (a.cu_q) {
+    q.q0 = __ldg(a.cu_q + b);
+    const int end = __ldg(a.cu_q + b + 1);
+    const bool falls = q.q0 < 0 || end < q.q0;
+    q.all = falls ? 0 : end - q.q0;
+    q.n = min(q.all, a.max_q);
+    if (err && (falls || q.all > a.max_q)) atomicCAS(err, 0, ROUGE_B200_EINVAL);
+  }
+  return q;
+}
+
 // First key a query at position p may see through the window.
 __device__ __forceinline__ int window_start(int p, int window) {
   return p < window ? 0 : p - window + 1;

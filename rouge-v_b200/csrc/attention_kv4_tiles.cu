@@ -121,9 +121,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
   const int per_seq = pairs * a.Hkv;
   const int b = blockIdx.x / per_seq, rem = blockIdx.x - b * per_seq;
   const int pair = pairs - 1 - rem / a.Hkv, hk = rem % a.Hkv;
-  const int q0 = a.cu_q ? __ldg(a.cu_q + b) : b;
-  const int n_all = a.cu_q ? __ldg(a.cu_q + b + 1) - q0 : 1;
-  const int nq = max(0, min(n_all, a.max_q)), nrows = nq * a.group;
+  const SeqQueries sq = seq_queries(a, b, a.err);
+  const int q0 = sq.q0, n_all = sq.all, nrows = sq.n * a.group;
   const int r0 = pair * kRows;
   if (r0 >= nrows) return;
   const int len_all = max(0, __ldg(a.kv_len + b)), p0 = len_all - n_all, len = min(len_all, a.max_kv);

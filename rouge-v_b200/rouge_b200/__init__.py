@@ -490,11 +490,12 @@ def attention_kv4_workspace(B, Hq, Hkv, Dh, max_q, max_kv, type):
     return lib().rouge_b200_attention_kv4_workspace(B, Hq, Hkv, Dh, max_q, max_kv, type)
 
 
-def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scale=0.0, causal=1,
+def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=None, O=None, scale=0.0, causal=1,
                   window=0, workspace=None):
     """O[T][Hq][Dh] of Q[T][Hq][Dh] over a KV4Cache: sequence b has kv_len[b] keys
     on the pages page_table[b] and the queries cu_q[b] .. cu_q[b + 1] (None: one
-    each). workspace: uint8, attention_kv4_workspace() bytes."""
+    each), at most max_q of them, which is required with cu_q: rows past the max_q-th
+    of a sequence are not computed, and sync_status() raises. workspace: uint8, attention_kv4_workspace() bytes."""
     import torch
     B, max_pages = page_table.shape
     T, Hq, Dh = Q.shape
@@ -509,10 +510,13 @@ def attention_kv4(Q, cache, kv_len, page_table, cu_q=None, max_q=1, O=None, scal
             not (kv_len.is_contiguous() and page_table.is_contiguous())):
         raise ValueError(f"contiguous int32 kv_len [{B}] and page_table [{B}, {max_pages}] expected")
     if cu_q is None:
-        if T < B or max_q != 1:
+        if T < B or max_q not in (None, 1):
             raise ValueError("without cu_q: one query per sequence")
+        max_q = 1
     elif cu_q.dtype != i32 or cu_q.shape != (B + 1,) or not cu_q.is_contiguous():
         raise ValueError(f"cu_q: contiguous int32 [{B + 1}] expected")
+    elif max_q is None and T > 0:
+        raise ValueError("max_q: the most queries of one sequence expected with cu_q")
     _check_device(Q, O, kv_len, page_table, cu_q, workspace, *cache.tensors)
     ty = _type_of(Q)
     if T == 0:  # (an empty tensor has no address)

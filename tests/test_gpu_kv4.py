@@ -642,3 +642,47 @@ def test_query_channels_far_above_the_others(rb, cuda, t, up, nq, Hq, Dh):
     rb.sync_status()
     hidden = torch.zeros(n, dtype=torch.bool, device="cuda")
     _close(O, *_sequence_reference(cache, q, n, table[0], 0, hidden, 2.0 ** -32 if nq == 400 else 2.0 ** -40), t, n)
+
+
+@pytest.mark.parametrize("t,Hq,Dh,page,counts,max_q", [("f32", 4, 64, 16, [3, 5, 2], 3), ("bf16", 8, 80, 16, [3, 1, 2], 1),
+                                                       ("bf16", 16, 128, 32, [300, 301, 7], 300)])
+def test_queries_past_max_q_are_reported(rb, cuda, t, Hq, Dh, page, counts, max_q):
+    """They are left as they were; the others keep their positions and values."""
+    import torch
+    n, Hkv, T = 320, 4, sum(counts)
+    cache = _cache(rb, 3 * n // page, Hkv, page, Dh, max_q)
+    table = torch.arange(3 * n // page, dtype=torch.int32, device="cuda").reshape(3, -1)
+    lens = torch.full((3,), n, dtype=torch.int32, device="cuda")
+    cu = torch.tensor(np.concatenate(([0], np.cumsum(counts))), dtype=torch.int32, device="cuda")
+    q = torch.randn(T, Hq, Dh, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(_dt(t))
+    want = rb.attention_kv4(q, cache, lens, table, cu_q=cu, max_q=max(counts))
+    rb.sync_status()
+    O = torch.full_like(q, 77.0)
+    rb.attention_kv4(q, cache, lens, table, cu_q=cu, max_q=max_q, O=O)
+    with pytest.raises(rb.RougeB200Error) as e:
+        rb.sync_status()
+    assert e.value.status == rb.EINVAL
+    done = torch.cat([torch.arange(c, device="cuda") < max_q for c in counts])
+    assert (O[~done] == 77).all()
+    # (another max_q may take another kernel: equal up to both kernels' roundings of weights and output)
+    assert torch.allclose(O[done].float(), want[done].float(), rtol=0, atol=2.0 ** -6)
+
+
+@pytest.mark.parametrize("t,Hq,Dh,max_q", [("f32", 4, 64, 3), ("bf16", 16, 128, 400)])
+def test_query_offsets_that_fall_are_reported(rb, cuda, t, Hq, Dh, max_q):
+    """Sequences whose offsets fall or are negative are left out; the others are computed."""
+    import torch
+    cache = _cache(rb, 40, 4, 16, Dh, 2)
+    table = torch.arange(40, dtype=torch.int32, device="cuda").reshape(4, 10)
+    lens = torch.full((4,), 160, dtype=torch.int32, device="cuda")
+    q = torch.randn(9, Hq, Dh, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(_dt(t))
+    run = lambda cu, O: rb.attention_kv4(q, cache, lens, table, max_q=max_q, O=O,  # noqa: E731
+                                         cu_q=torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    want = run([0, 3, 3, 3, 6], torch.full_like(q, 77.0))
+    rb.sync_status()
+    for cu in ([0, 3, 1, 3, 6], [-2, 0, 3, 3, 6], [-2147483648, 0, 3, 3, 6], [2147483647, 0, 3, 3, 6]):
+        O = run(cu, torch.full_like(q, 77.0))
+        with pytest.raises(rb.RougeB200Error) as e:
+            rb.sync_status()
+        assert e.value.status == rb.EINVAL
+        assert torch.equal(O[3:], want[3:])

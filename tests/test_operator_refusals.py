@@ -167,3 +167,13 @@ def test_python_checks(rb):
             rb.add_rmsnorm_quant(z(4, 64), None, a["w"], 1e-5, 0, a["codes"], a["scales"])
     with pytest.raises(ValueError):
         rb.add_rmsnorm_quant(z(4, 64), z(4, 32), z(64), 1e-5, 0, z(4, 64, dtype=torch.int8), z(4), z(4, 64))
+
+
+def test_ragged_queries_need_max_q(rb):
+    import torch
+    z, i32 = torch.zeros, torch.int32
+    c = rb.KV4Cache.empty(2, 1, 16, 64, device="cpu")
+    with pytest.raises(ValueError, match="max_q"):
+        rb.attention_kv4(z(4, 4, 64), c, z(2, dtype=i32), z(2, 1, dtype=i32), cu_q=z(3, dtype=i32))
+    with pytest.raises(ValueError, match="one query"):
+        rb.attention_kv4(z(2, 4, 64), c, z(2, dtype=i32), z(2, 1, dtype=i32), max_q=2)
