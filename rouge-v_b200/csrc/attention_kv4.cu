@@ -66,7 +66,7 @@ struct SeqInfo {
 // Work of sequence b for row tiles of `rows` rows.
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs &a, int b, int rows) {
   SeqInfo s;
-  const SeqQueries q = seq_queries(a, b, a.err);
+  const SeqQueries q = seq_queries(a, b);
   s.q0 = q.q0;
   s.nq = q.n;
   s.len = max(0, __ldg(a.kv_len + b));
@@ -713,8 +713,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
     rt = a.by_heads.div(u.y);
     hk = u.y - rt * a.Hkv;
   }
-  const SeqQueries sq = seq_queries(a, b, nullptr);
-  const int q0 = sq.q0, nq = sq.n;
+  const int q0 = a.cu_q ? a.cu_q[b] : b;
+  int nq = a.cu_q ? a.cu_q[b + 1] : b + 1;
+  nq = q0 < 0 ? 0 : max(0, min(nq - q0, a.max_q));  // (as seq_queries)
   const int share = rows / gridDim.y, first = blockIdx.y * share;
   const int live = min(share, nq * a.group - rt * rows - first);  // this block's rows
   if (live <= 0 || u.w < 2) return;

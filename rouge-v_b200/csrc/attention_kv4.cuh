@@ -44,11 +44,11 @@ namespace {
 
 // The queries of sequence b: first row, their number (all of them, and those
 // that are computed). More than max_q, or offsets that fall or start below
-// zero, are reported to `err` where it is given.
+// zero, are reported.
 struct SeqQueries {
   int q0, all, n;
 };
-__device__ __forceinline__ SeqQueries seq_queries(const AttnArgs &a, int b, int *err) {
+__device__ __forceinline__ SeqQueries seq_queries(const AttnArgs &a, int b) {
   SeqQueries q{b, 1, 1};
   if (a.cu_q) {
     q.q0 = __ldg(a.cu_q + b);
@@ -56,7 +56,7 @@ __device__ __forceinline__ SeqQueries seq_queries(const AttnArgs &a, int b, int 
     const bool falls = q.q0 < 0 || end < q.q0;
     q.all = falls ? 0 : end - q.q0;
     q.n = min(q.all, a.max_q);
-    if (err && (falls || q.all > a.max_q)) atomicCAS(err, 0, ROUGE_B200_EINVAL);
+    if (falls || q.all > a.max_q) atomicCAS(a.err, 0, ROUGE_B200_EINVAL);
   }
   return q;
 }

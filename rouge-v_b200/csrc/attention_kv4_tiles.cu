@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
   const int per_seq = pairs * a.Hkv;
   const int b = blockIdx.x / per_seq, rem = blockIdx.x - b * per_seq;
   const int pair = pairs - 1 - rem / a.Hkv, hk = rem % a.Hkv;
-  const SeqQueries sq = seq_queries(a, b, a.err);
+  const SeqQueries sq = seq_queries(a, b);
   const int q0 = sq.q0, n_all = sq.all, nrows = sq.n * a.group;
   const int r0 = pair * kRows;
   if (r0 >= nrows) return;
