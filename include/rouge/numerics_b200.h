@@ -672,23 +672,26 @@ int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void 
  * page_table[b * max_pages + t / page] * page + t % page, and the queries
  * cu_q[b] .. cu_q[b + 1] (device int32 [B + 1], ascending from 0, the last
  * at most the rows of Q; NULL: one query per sequence), at most max_q of
- * them. Q, O [cu_q[B]][Hq][Dh] of `type`, contiguous, 16-byte aligned. Query i of n sits at key position
- * s = kv_len[b] - n + i: causal masks t > s, window > 0 masks
- * t < s - window + 1. scale <= 0 means 1 / sqrt(Dh). Queries with no key
- * left give 0; rows of O past cu_q[B] are left as they were. Scores, softmax
- * and sums in f32. f32 queries are held to 2^-23 of each value (or 2^-50 of
- * their row's largest), f16 ones exactly, bf16 ones exactly (or to 2^-40 of
- * the largest); softmax weights to 2^-23 for f32 and 2^-11 for the 16-bit
- * types (or, of the largest weight, 2^-40, in long prompt chunks 2^-32).
+ * them. Q, O [cu_q[B]][Hq][Dh] of `type`, contiguous, 16-byte aligned, apart
+ * from each other. Query i of n sits at key position s = kv_len[b] - n + i:
+ * causal masks t > s, window > 0 masks t < s - window + 1. scale <= 0 means
+ * 1 / sqrt(Dh). Queries with no key left give 0; rows of O past cu_q[B] are
+ * left as they were. Scores, softmax and sums in f32. f32 queries are held to
+ * 2^-23 of each value (or 2^-50 of their row's largest), f16 ones exactly, bf16
+ * ones exactly (or to 2^-40 of the largest); softmax weights to 2^-23 for f32
+ * and 2^-11 for the 16-bit types (or, of the largest weight, 2^-40, in long
+ * prompt chunks 2^-32).
  * Limits, after which the next rouge_b200_sync_status returns
  * ROUGE_B200_EINVAL: of a sequence with more than max_q queries the first
  * max_q are computed, the others' rows of O are left as they were (of one
  * whose cu_q falls or is negative, all); key positions past max_pages * page
  * (below 2^31 - 1023), or on a page number outside the cache, are taken as
- * masked. The workspace
- * (rouge_b200_attention_kv4_workspace bytes, 256-byte aligned, no
- * initialisation) belongs to the call until it has finished: calls that may
- * run at the same time, captured graphs among them, each need their own. */
+ * masked.
+ * The workspace (256-byte aligned, no initialisation) has the bytes that
+ * rouge_b200_attention_kv4_workspace gives for the call's sizes, max_kv being
+ * max_pages * page (0 for sizes that the call refuses); it belongs to the
+ * call until it has finished: calls that may run at the same time, captured
+ * graphs among them, each need their own. */
 size_t rouge_b200_attention_kv4_workspace(int B, int Hq, int Hkv, int Dh, int max_q, int max_kv,
                                           int type);
 int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type, int B, int Hq,

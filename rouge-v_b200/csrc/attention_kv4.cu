@@ -780,11 +780,11 @@ int rows_of(int group, int max_q, int type) {
 // mma column tiles per warp (see Shape).
 int nt_of(int rows, int type) { return type == ROUGE_B200_T_F32 || rows == 16 ? 2 : 1; }
 
-// Warps of the grid: every SM's, fewer where even the longest sequences
-// would leave warps idle.
-int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, int type) {
+// Warps of the grid on `sms` SMs: all they hold, fewer where even the longest
+// sequences would leave warps idle. Not fewer on more SMs.
+int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, int type, int sms) {
   const int rows = rows_of(group, max_q, type), nt = nt_of(rows, type), warps = warps_of(Dh, nt);
-  const int sms = current_sm_count(), cap = sms * ctas_of(Dh, nt) * warps;
+  const int cap = sms * ctas_of(Dh, nt) * warps;
   const double rts = std::ceil(static_cast<double>(group) * max_q / rows);
   const double tiles = max_kv < kTile ? 1.0 : std::ceil(static_cast<double>(max_kv) / kTile);
   const double all = static_cast<double>(B) * Hkv * rts * tiles;
@@ -796,6 +796,13 @@ int grid_warps(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, i
 
 size_t part_bytes(int warps, int rows, int Dh) {
   return round_up(static_cast<size_t>(2) * warps * rows * (Dh + 4) * 4, 256);
+}
+
+// Workspace of a call on all of the device's SMs: a budget of fewer
+// (rouge_b200_set_sm_budget) may be set or lifted between sizing and call.
+size_t workspace_bytes_of(int B, int Hkv, int group, int Dh, int max_q, long long max_kv, int type) {
+  const int warps = grid_warps(B, Hkv, group, Dh, max_q, max_kv, type, device_sm_count());
+  return part_bytes(warps, rows_of(group, max_q, type), Dh) + static_cast<size_t>(warps) * 16;
 }
 
 template <int DT, int NT, int T, bool FULL>
@@ -861,8 +868,7 @@ size_t rouge_b200_attention_kv4_workspace(int B, int Hq, int Hkv, int Dh, int ma
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Dh <= 0 || Dh > 256 || max_q <= 0 ||
       max_kv <= 0 || !valid_float_type(type) || device_ready() != ROUGE_B200_OK)
     return 0;
-  const int warps = grid_warps(B, Hkv, Hq / Hkv, Dh, max_q, max_kv, type);
-  return part_bytes(warps, rows_of(Hq / Hkv, max_q, type), Dh) + static_cast<size_t>(warps) * 16;
+  return workspace_bytes_of(B, Hkv, Hq / Hkv, Dh, max_q, max_kv, type);
 }
 
 int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type, int B, int Hq,
@@ -896,13 +902,13 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   a.causal = causal;
   a.window = window < max_kv ? window : 0;  // (a window past the table hides nothing)
   const int rt_rows = rows_of(a.group, max_q, type);
-  a.warps = grid_warps(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type);
+  a.sms = current_sm_count();
+  a.warps = grid_warps(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type, a.sms);
   const size_t pb = part_bytes(a.warps, rt_rows, a.Dh);
-  if (!workspace || workspace_bytes < pb + static_cast<size_t>(a.warps) * 16)
+  if (!workspace || workspace_bytes < workspace_bytes_of(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type))
     return set_status(ROUGE_B200_ETOOBIG);
   a.part = static_cast<float *>(workspace);
   a.joins = reinterpret_cast<int4 *>(static_cast<uint8_t *>(workspace) + pb);
-  a.sms = current_sm_count();
   a.row_tiles = static_cast<int>((rows + rt_rows - 1) / rt_rows);
   a.by_unit = static_cast<double>(B) * a.Hkv * a.row_tiles < a.warps ? 1 : 0;
   a.by_group = Divisor(a.group);

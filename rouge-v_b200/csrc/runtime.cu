@@ -131,10 +131,13 @@ int current_device() {
   return current_device_index(&dev) == ROUGE_B200_OK ? dev : 0;
 }
 
-int current_sm_count() {
+int device_sm_count() {
   int dev = 0;
-  if (current_device_index(&dev) != ROUGE_B200_OK) return 0;
-  const int n = devices()[dev].sm_count;
+  return current_device_index(&dev) == ROUGE_B200_OK ? devices()[dev].sm_count : 0;
+}
+
+int current_sm_count() {
+  const int n = device_sm_count();
   const int cap = g_sm_budget.load();
   return (cap > 0 && cap < n) ? cap : n;
 }

@@ -26,6 +26,9 @@ int device_ready();
 // Index (below 64) of the current device; 0 if it cannot be read.
 int current_device();
 int current_sm_count();
+// All SMs of the current device, whatever rouge_b200_set_sm_budget says (for
+// sizes that must not change between two calls).
+int device_sm_count();
 
 // Device word (int) that kernels set to a non-zero status when a bounded
 // wait gives up. One per device, allocated on first use.

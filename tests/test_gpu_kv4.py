@@ -686,3 +686,28 @@ def test_query_offsets_that_fall_are_reported(rb, cuda, t, Hq, Dh, max_q):
             rb.sync_status()
         assert e.value.status == rb.EINVAL
         assert torch.equal(O[3:], want[3:])
+
+
+def test_workspace_does_not_depend_on_the_sm_budget(rb, cuda):
+    """Sized under one budget of SMs and used under another."""
+    import torch
+    cache = _cache(rb, 200, 2, 16, 64, 5)
+    q = torch.randn(3, 8, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    lens = torch.tensor([1000, 3, 1056], dtype=torch.int32, device="cuda")
+    table = torch.arange(198, dtype=torch.int32, device="cuda").reshape(3, 66)
+    size = lambda: rb.attention_kv4_workspace(3, 8, 2, 64, 1, 1056, rb.T_F32)  # noqa: E731
+    n = size()
+    L = rb.lib()
+    old = L.rouge_b200_set_sm_budget(5)
+    try:
+        small = size()
+        assert small == n
+        ws = torch.empty(small, dtype=torch.uint8, device="cuda")
+        few = rb.attention_kv4(q, cache, lens, table, workspace=ws).clone()
+    finally:
+        L.rouge_b200_set_sm_budget(old)
+    all_ = rb.attention_kv4(q, cache, lens, table, workspace=ws)
+    rb.sync_status()
+    want, spread, ds, tiny = _reference(cache, q, [1000, 3, 1056], table, [1, 1, 1], 1, 0, 1 / 8)
+    _close(few, want, spread, ds, tiny, "f32", 1056)
+    _close(all_, want, spread, ds, tiny, "f32", 1056)
