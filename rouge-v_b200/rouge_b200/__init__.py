@@ -577,6 +577,11 @@ def _check_device(*tensors):
             raise ValueError(f"tensor on {t.device}, current device cuda:{dev}")
 
 
+def _pitch(t):
+    """Row pitch of a matrix with contiguous rows (a single row's stride can be any)."""
+    return max(t.stride(0), t.shape[-1]) if t.shape[0] < 2 else t.stride(0)
+
+
 class Epilogue:
     """Epilogue of gemm_i8 / gemm_e4m3 / gemm_f16: act(. + bias[n]) + residual[m][n],
     each optional. bias: f32 [N]; residual: f32, f16 or bf16 [M][N], rows
@@ -586,7 +591,7 @@ class Epilogue:
         self.tensors = (bias, residual)  # (kept alive)
         self.c = _EpilogueC(None if bias is None else bias.data_ptr(),
                             None if residual is None else residual.data_ptr(),
-                            0 if residual is None else residual.stride(0),
+                            0 if residual is None else _pitch(residual),
                             T_F32 if residual is None else _type_of(residual), act)
         self.ref = C.byref(self.c)
 
@@ -602,15 +607,39 @@ class Epilogue:
         _check_device(bias, residual, *others)
 
 
+_out_types = {}
+
+
+def _fused_sizes(epilogue, A, B, b_layout, C_, out_type, esize, scale_a, na, scale_b, nb):
+    """Raises unless the tensors of a product with an epilogue have the sizes, element sizes and layouts
+    that the kernel reads and writes; na, nb: elements of the scales, None for M and N."""
+    import torch
+    if not _out_types:
+        _out_types.update({OUT_F32: torch.float32, OUT_BF16: torch.bfloat16})
+    M, K = A.shape
+    N = B.shape[1 if b_layout == B_KN else 0]
+    if B.shape[0 if b_layout == B_KN else 1] != K or not (A.is_contiguous() and B.is_contiguous()):
+        raise ValueError(f"contiguous A [M, K] and B {'[K, N]' if b_layout == B_KN else '[N, K]'} expected")
+    if A.element_size() != esize or B.element_size() != esize:
+        raise ValueError(f"A, B: elements of {esize} bytes expected")
+    if C_.shape != (M, N) or (N > 1 and C_.stride(1) != 1) or C_.dtype != _out_types.get(out_type, C_.dtype):
+        raise ValueError(f"output: [{M}, {N}] of out_type with contiguous rows expected")
+    for t, n in ((scale_a, M if na is None else na), (scale_b, N if nb is None else nb)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous()):
+            raise ValueError(f"scales: {n} contiguous float32 expected")
+    epilogue.check(M, N, A, B, C_, scale_a, scale_b)
+
+
 def gemm_i8(A, B, b_layout, C_, out_type, scales_a=None, a_rows=1, scales_b=None, b_cols=1,
             epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N, A, B, C_)
+        _fused_sizes(epilogue, A, B, b_layout, C_, out_type, 1, scales_a, None if a_rows else 1, scales_b,
+                     None if b_cols else 1)
         _check("rouge_b200_gemm_i8_fused", lib().rouge_b200_gemm_i8_fused(
             M, N, K, _ptr(A), _ptr(B), b_layout, _ptr(scales_a), a_rows, _ptr(scales_b), b_cols,
-            epilogue.ref, _ptr(C_), C_.stride(0), out_type, _stream()))
+            epilogue.ref, _ptr(C_), _pitch(C_), out_type, _stream()))
         return
     _check("rouge_b200_gemm_i8", lib().rouge_b200_gemm_i8(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scales_a), a_rows, _dp(scales_b), b_cols,
@@ -653,10 +682,10 @@ def gemm_e4m3(A, B, b_layout, C_, out_type, scale_a=None, scale_b=None, epilogue
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N, A, B, C_)
+        _fused_sizes(epilogue, A, B, b_layout, C_, out_type, 1, scale_a, 1, scale_b, 1)
         _check("rouge_b200_gemm_e4m3_fused", lib().rouge_b200_gemm_e4m3_fused(
             M, N, K, _ptr(A), _ptr(B), b_layout, _ptr(scale_a), _ptr(scale_b), epilogue.ref,
-            _ptr(C_), C_.stride(0), out_type, _stream()))
+            _ptr(C_), _pitch(C_), out_type, _stream()))
         return
     _check("rouge_b200_gemm_e4m3", lib().rouge_b200_gemm_e4m3(
         M, N, K, _dp(A), _dp(B), b_layout, _dp(scale_a), _dp(scale_b), _dp(C_), C_.stride(0),
@@ -667,10 +696,10 @@ def gemm_f16(A, B, b_layout, C_, out_type, is_bf16=False, epilogue=None):
     M, K = A.shape
     N = B.shape[1] if b_layout == B_KN else B.shape[0]
     if epilogue is not None:
-        epilogue.check(M, N, A, B, C_)
+        _fused_sizes(epilogue, A, B, b_layout, C_, out_type, 2, None, 1, None, 1)
         _check("rouge_b200_gemm_f16_fused", lib().rouge_b200_gemm_f16_fused(
             M, N, K, _ptr(A), _ptr(B), b_layout, int(is_bf16), epilogue.ref, _ptr(C_),
-            C_.stride(0), out_type, _stream()))
+            _pitch(C_), out_type, _stream()))
         return
     _check("rouge_b200_gemm_f16", lib().rouge_b200_gemm_f16(
         M, N, K, _dp(A), _dp(B), b_layout, int(is_bf16), _dp(C_), C_.stride(0), out_type,

@@ -177,3 +177,47 @@ def test_ragged_queries_need_max_q(rb):
         rb.attention_kv4(z(4, 4, 64), c, z(2, dtype=i32), z(2, 1, dtype=i32), cu_q=z(3, dtype=i32))
     with pytest.raises(ValueError, match="one query"):
         rb.attention_kv4(z(2, 4, 64), c, z(2, dtype=i32), z(2, 1, dtype=i32), max_q=2)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3", "f16", "bf16"])
+@pytest.mark.parametrize("layout", [0, 1])
+def test_fused_gemm_tensors_are_checked(rb, kind, layout):
+    """Anything the kernel would read or write past a tensor's end, or take for another type."""
+    import torch
+    M, N, K = 8, 48, 32
+    dt = dict(i8=torch.int8, e4m3=torch.float8_e4m3fn, f16=torch.float16, bf16=torch.bfloat16)[kind]
+    z = torch.zeros
+    B = (K, N) if layout == 0 else (N, K)
+    good = dict(A=z(M, K, dtype=dt), B=z(B, dtype=dt), C=z(M, N), out=rb.OUT_F32, sa=z(M), sb=z(N), rows=1, cols=1,
+                ep=rb.Epilogue(z(N), 0, z(M, N)))
+
+    def call(**kw):
+        a = good | kw
+        if kind == "i8":
+            rb.gemm_i8(a["A"], a["B"], layout, a["C"], a["out"], a["sa"], a["rows"], a["sb"], a["cols"],
+                       epilogue=a["ep"])
+        elif kind == "e4m3":
+            rb.gemm_e4m3(a["A"], a["B"], layout, a["C"], a["out"], a["sa"], a["sb"], epilogue=a["ep"])
+        else:
+            rb.gemm_f16(a["A"], a["B"], layout, a["C"], a["out"], kind == "bf16", epilogue=a["ep"])
+
+    bad = [dict(C=z(M, N, dtype=torch.bfloat16)), dict(out=rb.OUT_BF16), dict(C=z(M, N, dtype=torch.float64)),
+           dict(C=z(M - 1, N)), dict(C=z(M, N - 1)), dict(C=z(M, 2 * N)[:, ::2]), dict(C=z(N, M).T),
+           dict(A=z(M, 2 * K, dtype=dt)[:, :K]), dict(A=z(M, K + 16, dtype=dt)), dict(A=z(M, K)),
+           dict(B=z(B)), dict(B=z(B[::-1], dtype=dt).T), dict(B=z(B[0] + (layout == 0), B[1] + layout, dtype=dt)),
+           dict(ep=rb.Epilogue(z(N + 1))), dict(ep=rb.Epilogue(residual=z(M, N + 1)))]
+    if kind == "i8":
+        bad += [dict(sa=z(M - 1)), dict(sb=z(N - 1)), dict(sa=z(2 * M)[::2]), dict(sb=z(N, dtype=torch.float64)),
+                dict(sa=z(0), rows=0), dict(sb=z(0), cols=0)]
+    if kind == "e4m3":
+        bad += [dict(sa=z(0)), dict(sb=z(1, dtype=torch.float16))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            call(**kw)
+
+
+def test_pitch_of_one_row(rb):
+    import torch
+    row = torch.zeros(64, 1).T  # [1, 64] whose row stride is 1
+    assert row.stride(0) == 1 and rb.Epilogue(residual=row).c.ldr == 64
+    assert rb.Epilogue(residual=torch.zeros(3, 80)[:, :64]).c.ldr == 80
