@@ -640,7 +640,7 @@ int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const void *resid
  * block, 4.5 bits per value; value = code * scale * gs[head].
  *   k_codes, v_codes    [pages][Hkv][page][Dh / 2]   bytes
  *   k_scales, v_scales  [pages][Hkv][page][Dh / 16]  bytes
- *   gs_k, gs_v          [Hkv] f32 > 0, or NULL for 1
+ *   gs_k, gs_v          [Hkv] f32 > 0 with 6 gs finite, or NULL for 1
  * page a multiple of 16, Dh a multiple of 16 up to 256, arrays 16-byte
  * aligned, pages * page below 2^31; otherwise ROUGE_B200_EUNSUPPORTED. All
  * pointers are device pointers; the struct itself is read before a call

@@ -128,8 +128,8 @@ __device__ __forceinline__ bool locate(const KvArgs &a, unsigned i, int &head, l
 
 // Quotients x / step for the codes' border tests, correctly rounded: one
 // Newton step on the product with the reciprocal, whose residual is exact
-// while nothing under- or overflows; a quotient that is exactly a border
-// between two codes is then met exactly.
+// while nothing under- or overflows (quotients up to 2^24 here); a quotient
+// that is exactly a border between two codes is then met exactly.
 __device__ __forceinline__ void quotients(float &x, float &y, float step, float inv) {
   float q0, q1, r0, r1;
   mul2(q0, q1, x, y, inv);
@@ -138,7 +138,8 @@ __device__ __forceinline__ void quotients(float &x, float &y, float step, float 
 }
 
 // The same for one value of a block that holds an infinity or a NaN, or whose
-// step is extreme (infinities divide to infinities, NaN stays).
+// step or largest quotient (where the scale has saturated) is extreme:
+// infinities divide to infinities, as do quotients too large, NaN stays.
 __device__ __forceinline__ float quotient_any(float x, float step) { return __fdiv_rn(x, step); }
 
 // Clears the sign of zero codes (the hardware keeps it; eight nibbles).
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const KvArgs a) {
     const float step = __fmul_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(sh))), g);
     uint2 w = make_uint2(0u, 0u);
     if (step > 0.0f) {
-      if (odd || !(step > 7.9e-31f && step < 1.2e30f)) {
+      if (odd || !(step > 7.9e-31f && step < 1.2e30f) || m > 16777216.0f * step) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = quotient_any(v[j], step);
       } else {

@@ -711,3 +711,23 @@ def test_workspace_does_not_depend_on_the_sm_budget(rb, cuda):
     want, spread, ds, tiny = _reference(cache, q, [1000, 3, 1056], table, [1, 1, 1], 1, 0, 1 / 8)
     _close(few, want, spread, ds, tiny, "f32", 1056)
     _close(all_, want, spread, ds, tiny, "f32", 1056)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("g", [2.0 ** -10, 1e-30, 1e20])
+def test_write_saturates_with_the_sign(rb, cuda, t, g):
+    """Values so far above 448 * 6 * gs that their quotient by the block's step leaves f32's range."""
+    import torch
+    gs = torch.tensor([g], device="cuda")
+    cache = rb.KV4Cache.empty(1, 1, 16, 32, gs, gs)
+    top = torch.finfo(torch.bfloat16).max
+    K = torch.zeros(3, 1, 32, device="cuda")
+    K[0, 0, :8] = torch.tensor([top, -top, top / 2, -top / 2, 1.0, -1.0, -1e30, 1e30])
+    K[1, 0, 16:20] = torch.tensor([-top, 3 * g, -6 * 448 * g, 448 * g])
+    K[2, 0, :4] = torch.tensor([-1e9, 1e9, -1e-3, 0.0])
+    x = K.to(_dt(t))
+    rb.kv4_write(cache, x, x, torch.arange(3, dtype=torch.int32, device="cuda"))
+    rb.sync_status()
+    c, s = _quantize(x, gs[None, :, None])
+    for codes, scales in (cache.tensors[:2], cache.tensors[2:4]):
+        assert torch.equal(scales[0, 0, :3], s[:, 0]) and torch.equal(codes[0, 0, :3], c[:, 0])
