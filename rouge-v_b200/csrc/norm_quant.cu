@@ -4,8 +4,10 @@
 //   codes, scales = per-row int8 (quant_int8.cpp:72-90) or MXFP8 e4m3
 //                   blocks of 32 (narrow.cpp:200-265) of y
 // with the arithmetic of those steps apart: sum of squares and inverse root
-// in double, the scaled product rounded once (norm_value), so the codes are
-// those of rouge_rmsnorm followed by the quantizer.
+// in double, the scaled product rounded once (norm_values), so the codes are
+// those of rouge_rmsnorm followed by the quantizer, unless the scaled product
+// lies within about 2^-47 of itself of the middle of two floats (the sum of
+// squares is added up in another order). The sign of a NaN is not kept.
 //
 // Memory-bound: a row is read once and stays in registers (16 values per
 // thread) over both reductions -- the sum of squares, then the row maximum
@@ -124,7 +126,9 @@ __device__ __forceinline__ void group_sync(int id, int threads) {
 }
 
 // The row's inverse root mean square: the double, and its two leading floats
-// (hi + lo = the double to 2^-48; hi infinite where the double is too large).
+// (hi + lo = the double to 2^-48). hi is infinite where two floats do not
+// serve: where the double or its lower part leaves f32's normal range, and
+// where the row is so small that its outputs or their remainders may.
 struct InvRms {
   double full;
   float hi, lo;
@@ -134,8 +138,11 @@ struct InvRms {
 // approximation (2^-22, 2^-43, 2^-53), in a chain a third as long as double
 // division, root and division; those serve for values out of f32's range.
 __device__ __forceinline__ InvRms inverse_rms(double ss, double by_n, float eps) {
-  const double v = __dadd_rn(__dmul_rn(ss, by_n), static_cast<double>(eps));
+  const double mean = __dmul_rn(ss, by_n);
+  const double v = __dadd_rn(mean, static_cast<double>(eps));
   InvRms r;
+  // 0 < mean < 2^-180 by its high word (a row of zeros is zeros either way)
+  bool two_floats = static_cast<unsigned>(__double2hiint(mean) - 1) >= ((1023u - 180u) << 20) - 1u;
   if (v > 1e-30 && v < 1e30) {
     double y = static_cast<double>(rsqrtf(__double2float_rn(v)));
 #pragma unroll
@@ -146,9 +153,11 @@ __device__ __forceinline__ InvRms inverse_rms(double ss, double by_n, float eps)
     r.full = y;
   } else {
     r.full = __ddiv_rn(1.0, __dsqrt_rn(v));
+    two_floats = two_floats && !(r.full < 7.9e-31);  // 2^-100
   }
   r.hi = __double2float_rn(r.full);
   r.lo = __double2float_rn(__dsub_rn(r.full, static_cast<double>(r.hi)));
+  if (!two_floats) r.hi = INFINITY;
   return r;
 }
 
@@ -160,7 +169,7 @@ __device__ __forceinline__ InvRms inverse_rms(double ss, double by_n, float eps)
 // of two floats.
 template <int V>
 __device__ __forceinline__ void norm_values(float (&h)[V], const InvRms &inv, const float (&w)[V]) {
-  if (isinf(inv.hi)) {  // (rows of subnormals without eps, NaN for zero rows)
+  if (isinf(inv.hi)) {  // (for rows of zeros without eps: NaN)
 #pragma unroll
     for (int j = 0; j < V; ++j)
       h[j] = __fmul_rn(__double2float_rn(__dmul_rn(static_cast<double>(h[j]), inv.full)), w[j]);

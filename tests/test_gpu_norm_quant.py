@@ -154,3 +154,53 @@ def test_no_rows_and_rows_behind(rb, cuda):
     rb.add_rmsnorm_quant(x, None, torch.ones(64, device="cuda"), 1e-5, 0, codes, scales)
     rb.sync_status()
     assert (codes[4:] == 77).all() and (scales[4:] == 7).all() and (scales[:4] != 7).all()
+
+
+def _separate_steps(rb, h, w, eps):
+    """int8 codes and scales, MXFP8 codes and scales of rouge_rmsnorm followed by the quantizers."""
+    import ctypes as C
+
+    import torch
+    L = rb.lib()
+    L.rouge_rmsnorm.argtypes, L.rouge_rmsnorm.restype = [C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p], None
+    x, wn = np.ascontiguousarray(h.float().cpu().numpy()), w.cpu().numpy()
+    y = np.empty_like(x)
+    p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    for i in range(x.shape[0]):
+        L.rouge_rmsnorm(p(x[i]), x.shape[1], p(wn), eps, p(y[i]))
+    yd = torch.from_numpy(y).cuda()
+    rows, cols = y.shape
+    q, s = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    rb.quantize_i8_rows(yd, s, q)
+    m, e = torch.empty(rows, cols, dtype=torch.uint8, device="cuda"), torch.empty(rows, cols // 32, dtype=torch.uint8,
+                                                                                  device="cuda")
+    rb.mx_quantize(yd, rb.FMT_E4M3, m, e)
+    return q, s, m, e
+
+
+@pytest.mark.parametrize("scale", [1e30, 1e33, 1e36, 2e38, 1e-30, 1e-37, 1e-40, 1e-43])
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+def test_rows_at_the_ends_of_f32(rb, cuda, scale, eps):
+    """Rows whose inverse root leaves f32's normal range, or whose outputs do: still the separate steps' codes."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(9)
+    x = (0.4 + 1.2 * torch.rand(300, 512, generator=g, device="cuda")) * scale
+    x = torch.where(torch.rand(x.shape, generator=g, device="cuda") < 0.5, x, -x)
+    w = 0.5 + torch.rand(512, generator=g, device="cuda")
+    q, s, m, e = _separate_steps(rb, x, w, eps)
+    _, c0, s0 = _run(rb, x, None, w, 0, eps)
+    _, c1, s1 = _run(rb, x, None, w, 1, eps)
+    assert torch.equal(s0, s) and torch.equal(c0, q) and torch.equal(c1, m) and torch.equal(s1, e)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("cols", [96, 5120, 16416])
+def test_equals_the_separate_steps_with_residual(rb, cuda, t, cols):
+    import torch
+    g = torch.Generator("cuda").manual_seed(cols)
+    x, r = ((3 * torch.randn(9, cols, generator=g, device="cuda")).to(_dt(t)) for _ in range(2))
+    w = 0.5 + torch.rand(cols, generator=g, device="cuda")
+    q, s, m, e = _separate_steps(rb, (x.float() + r.float()).to(x.dtype), w, 1e-5)
+    _, c0, s0 = _run(rb, x, r, w, 0)
+    _, c1, s1 = _run(rb, x, r, w, 1)
+    assert torch.equal(s0, s) and torch.equal(c0, q) and torch.equal(c1, m) and torch.equal(s1, e)
