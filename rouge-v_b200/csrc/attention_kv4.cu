@@ -707,6 +707,10 @@ __global__ void __launch_bounds__(kJoinThreads) attention_kv4_join_kernel(const 
   }
   grid_dependency_wait();
   const int4 u = __ldcg(a.joins + blockIdx.x);
+  // (an entry by unit may not have been written: for a unit without rows, or
+  // when a wait of the first kernel ran out. No part outside the workspace is
+  // read, whatever it holds.)
+  if (u.z < 0 || u.w > a.warps - u.z) return;
   if (!a.by_unit) {
     if (u.w < 2) return;
     b = u.x;

@@ -731,3 +731,26 @@ def test_write_saturates_with_the_sign(rb, cuda, t, g):
     c, s = _quantize(x, gs[None, :, None])
     for codes, scales in (cache.tensors[:2], cache.tensors[2:4]):
         assert torch.equal(scales[0, 0, :3], s[:, 0]) and torch.equal(codes[0, 0, :3], c[:, 0])
+
+
+@pytest.mark.parametrize("B,nq", [(1, 1), (5, 1), (5, 3), (300, 1), (40, 20)])
+def test_workspace_needs_no_initialisation(rb, cuda, B, nq):
+    """Whatever bytes it holds, also for sequences without queries, whose units nothing writes."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(B)
+    cache = _cache(rb, 128, 2, 16, 64, B)
+    lens = torch.randint(0, 2049, (B,), generator=g, device="cuda").int()
+    table = torch.randint(0, 128, (B, 128), generator=g, device="cuda").int()
+    counts = torch.randint(0, nq + 1, (B,), generator=g, device="cuda") if nq > 1 else torch.ones(B, device="cuda")
+    cu = torch.cat((torch.zeros(1, device="cuda"), counts.cumsum(0))).int()
+    q = torch.randn(B * nq, 8, 64, generator=g, device="cuda").bfloat16()
+    ws = torch.zeros(rb.attention_kv4_workspace(B, 8, 2, 64, nq, 2048, rb.T_BF16), dtype=torch.uint8, device="cuda")
+    outs = []
+    for fill in (0, 0x7F, 0xFF, 0x01):
+        ws.fill_(fill)
+        O = torch.full_like(q, 77.0)
+        rb.attention_kv4(q, cache, lens, table, cu_q=cu, max_q=nq, O=O, workspace=ws)
+        rb.sync_status()
+        outs.append(O)
+    assert all(torch.equal(o, outs[0]) for o in outs) and (outs[0][cu[-1]:] == 77).all()
+    assert outs[0].isfinite().all()
