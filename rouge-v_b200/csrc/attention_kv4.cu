@@ -888,6 +888,8 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   const long long rows = static_cast<long long>(Hq / cache->Hkv) * max_q;
   if (max_kv > 0x7ffffc00LL || rows > 0x7ffffc00LL ||
       ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(O)) & 15u) ||
+      ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(kv_len) |
+        reinterpret_cast<uintptr_t>(page_table)) & 3u) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return set_status(ROUGE_B200_EUNSUPPORTED);
   s = device_ready();

@@ -221,3 +221,8 @@ def test_pitch_of_one_row(rb):
     row = torch.zeros(64, 1).T  # [1, 64] whose row stride is 1
     assert row.stride(0) == 1 and rb.Epilogue(residual=row).c.ldr == 64
     assert rb.Epilogue(residual=torch.zeros(3, 80)[:, :64]).c.ldr == 80
+
+
+@pytest.mark.parametrize("name", ["cu_q", "kv_len", "table"])
+def test_attention_misaligned_indices_refused(rb, call, name):
+    assert call("rouge_b200_attention_kv4", *_attn(rb, **{name: A + 2})) == rb.EUNSUPPORTED
