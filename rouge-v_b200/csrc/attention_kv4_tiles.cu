@@ -318,15 +318,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv4_tiles_kernel(const 
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0u;
         }
-        if (!live) continue;
+        if (live) {  // (the whole warp loads TMEM in the next round)
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float v[4];
+          for (int i = 0; i < 32; i += 4) {
+            float v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // (a row without keys: O may hold anything times zero)
-            v[k] = f == 0.0f ? 0.0f : __uint_as_float(y[i + k]) * f;
-          store_o4<T>(a.O, at + 32 * c + i, v[0], v[1], v[2], v[3]);
+            for (int k = 0; k < 4; ++k)  // (a row without keys: O may hold anything times zero)
+              v[k] = f == 0.0f ? 0.0f : __uint_as_float(y[i + k]) * f;
+            store_o4<T>(a.O, at + 32 * c + i, v[0], v[1], v[2], v[3]);
+          }
         }
+        __syncwarp();
       }
     }
   } else if (warp < 12) {
