@@ -906,7 +906,7 @@ int rouge_b200_attention_kv4(const RougeB200KV4 *cache, const void *Q, int type,
   a.max_kv = static_cast<int>(max_kv);
   a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->Dh));
   a.causal = causal;
-  a.window = window < max_kv ? window : 0;  // (a window past the table hides nothing)
+  a.window = window;
   const int rt_rows = rows_of(a.group, max_q, type);
   a.sms = current_sm_count();
   a.warps = grid_warps(B, a.Hkv, a.group, a.Dh, max_q, max_kv, type, a.sms);

@@ -754,3 +754,21 @@ def test_workspace_needs_no_initialisation(rb, cuda, B, nq):
         outs.append(O)
     assert all(torch.equal(o, outs[0]) for o in outs) and (outs[0][cu[-1]:] == 77).all()
     assert outs[0].isfinite().all()
+
+
+@pytest.mark.parametrize("t,nq,Hq", [("f32", 1, 4), ("bf16", 3, 8), ("bf16", 500, 16)])
+def test_window_counts_from_the_length_past_the_table(rb, cuda, t, nq, Hq):
+    """A length past the table's 640 keys (reported): those with a page are visible where the window reaches them."""
+    import torch
+    n, have, window = 1100, 640, 700
+    cache = _cache(rb, 40, 4, 16, 64, 3)
+    table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(nq, Hq, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(nq)).to(_dt(t))
+    O = rb.attention_kv4(q, cache, torch.tensor([n], dtype=torch.int32, device="cuda"), table, max_q=nq, window=window,
+                         cu_q=torch.tensor([0, nq], dtype=torch.int32, device="cuda"))
+    with pytest.raises(rb.RougeB200Error):
+        rb.sync_status()
+    longer = torch.cat((table, torch.zeros(1, n // 16, dtype=torch.int32, device="cuda")), 1)
+    hidden = torch.arange(n, device="cuda") >= have
+    _close(O, *_sequence_reference(cache, q, n, longer[0], window, hidden, 2.0 ** -32 if nq == 500 else 2.0 ** -40), t,
+           have)
