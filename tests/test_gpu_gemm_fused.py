@@ -186,3 +186,23 @@ def test_captured_and_replayed(rb, cuda):
     graph.replay()
     torch.cuda.synchronize()
     _check(v, c, 1, None, r)
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 4096), (32, 8192, 1040), (33, 528, 512), (513, 1040, 512), (1000, 4128, 2064)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_empty_epilogue_gives_the_plain_entrys_bits(rb, cuda, kind, M, N, K, layout):
+    """Also where the fused entry takes another tile: sums of random products, in the same order."""
+    import torch
+    A, B, sa, sb, _, g = _operands(kind, M, N, K, layout, M)
+    if kind in ("bf16", "f16"):
+        A, B = (torch.randn(t.shape, generator=g, device="cuda").to(t.dtype) for t in (A, B))
+    c, d = (torch.empty(M, N, device="cuda") for _ in range(2))
+    _call(rb, kind, A, B, layout, c, sa, sb, rb.Epilogue())
+    if kind == "i8":
+        rb.gemm_i8(A, B, layout, d, rb.OUT_F32, sa, 1, sb, 1)
+    elif kind == "e4m3":
+        rb.gemm_e4m3(A, B, layout, d, rb.OUT_F32, sa, sb)
+    else:
+        rb.gemm_f16(A, B, layout, d, rb.OUT_F32, kind == "bf16")
+    assert torch.equal(c, d)
