@@ -621,7 +621,11 @@ int rouge_b200_transformer_block(int S, int D, int Hq, int Hkv, int Dq, int Dk, 
  *     ROUGE_B200_Q_I8_ROWS  rouge_b200_quantize_i8_rows of y: scales f32
  *                           [rows] (cols % 4 == 0)
  *     ROUGE_B200_Q_MX_E4M3  rouge_b200_mx_quantize(E4M3) of y: scales
- *                           uint8 [rows][cols / 32] (cols % 32 == 0)
+ *                           uint8 [rows][cols / 32] (cols % 32 == 0). Its
+ *                           scales are 2 or more: blocks below 448, as normed
+ *                           rows are, all have 2, and values below 2^-5 are
+ *                           e4m3 subnormals
+ *     (the sign of a NaN is not kept)
  * type: ROUGE_B200_T_F32, _F16 or _BF16, of x, residual and h_out, whose
  * rows need 16-byte alignment (8 bytes for the 16-bit types; 16 is faster);
  * w f32 [cols], 16-byte aligned. h_out may be x or residual itself, with
@@ -637,7 +641,9 @@ int rouge_b200_add_rmsnorm_quant(const void *x, long long ldx, const void *resid
  * counterpart; its caches are f32 or e4m3). Token slot p * page + i is
  * position i of page p. Per slot and K/V head, Dh values in blocks of 16:
  * packed e2m1 codes (lower index in the low nibble) and one UE4M3 scale per
- * block, 4.5 bits per value; value = code * scale * gs[head].
+ * block (0x00 .. 0x7E; rouge_b200_kv4_write stores no other byte. With the NaN
+ * 0x7F in a key that some query sees, rows that do not see it may be NaN too),
+ * 4.5 bits per value; value = code * scale * gs[head].
  *   k_codes, v_codes    [pages][Hkv][page][Dh / 2]   bytes
  *   k_scales, v_scales  [pages][Hkv][page][Dh / 16]  bytes
  *   gs_k, gs_v          [Hkv] f32 > 0 with 6 gs finite, or NULL for 1
@@ -687,6 +693,9 @@ int rouge_b200_kv4_read(const RougeB200KV4 *cache, void *K, long long ldk, void 
  * whose cu_q falls or is negative, all); key positions past max_pages * page
  * (below 2^31 - 1023), or on a page number outside the cache, are taken as
  * masked.
+ * Calls with long prompt chunks and sequences of one query are faster as two
+ * calls: the kernel is chosen for a call as a whole, by max_q, and the one for
+ * chunks does not divide a sequence's keys.
  * The workspace (256-byte aligned, no initialisation) has the bytes that
  * rouge_b200_attention_kv4_workspace gives for the call's sizes, max_kv being
  * max_pages * page (0 for sizes that the call refuses); it belongs to the

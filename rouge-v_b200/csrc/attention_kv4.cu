@@ -27,9 +27,12 @@
 // tiles, whose scores are added; the weights, times 2^15, are split the same
 // way. Accumulation is f32.
 //
-// What bounds it is instruction issue: 64 sequences of up to 8192 keys, Hq 64,
-// Hkv 8, Dh 128 take 98.5 us, 59 % of the copy rate, with 63 % of the issue
-// slots used, 16 warps per SM and about 740 instructions per 32-key tile.
+// 64 sequences of up to 8192 keys, Hq 64, Hkv 8, Dh 128 take 98.5 us, 59 % of the
+// copy rate, with about 740 instructions per 32-key tile, 16 warps per SM, 63 %
+// of the issue slots and 60 % of the integer pipe used: neither memory nor issue
+// is full, four warps a scheduler do not cover one another's dependent chains.
+// Rows past 8 (groups of 16 heads, several queries) take NT = 2, whose 168
+// registers spill at Dh 80 to 128 (164 to 296 bytes): Hq 128 139 us.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

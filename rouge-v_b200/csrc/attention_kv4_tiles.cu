@@ -24,8 +24,8 @@
 // What bounds it: 64 keys of both tiles take 2226 cycles at Dh 128, of which
 // the MMAs would be 1330 by the rates of single ones (51.7 cycles at N = 64,
 // 64 at N = 128) and the 16384 exponentials 1024 on 16 lanes a cycle; the rest
-// are the groups' starts. 2 x 512 queries of 32 heads over up to 4096 keys: 92
-// us, 557 TFLOP/s. code * scale is exact in f16; 16-bit queries are
+// are the groups' starts. 2 x 512 queries of 32 heads over up to 4096 keys: 93
+// us, 553 TFLOP/s. code * scale is exact in f16; 16-bit queries are
 // held as row_exponent says; weights are rounded to f16.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -451,7 +451,12 @@ int launch_tiles(const AttnArgs &a, int pairs, cudaStream_t st) {
 // From 24 tiles of 256 rows on the tensor cores win. Tiles against warps, Dh
 // 128, Hq 32, Hkv 8, 2000 keys: 6400 rows (200 queries) 54.5 and 52.7 us, 8192
 // rows 54 and 62, 25600 rows 55 and 125. 16 sequences of 16 queries: 46.3 and
-// 50.6. Fewer than 64 rows per unit would leave most of a tile empty.
+// 50.6. Fewer than 64 rows per unit would leave most of a tile empty. The
+// choice is made for the whole call, from max_q: a block walks all keys of its
+// rows, so sequences with few queries and long pasts in one call with a long
+// chunk are slow here (one query over 131072 keys 2.4 ms, 62 us by the warps;
+// 63 decoding sequences of 4096 keys beside a chunk of 512 364 us, 81 and 93 in
+// two calls), as is a chunk over so long a past (512 queries, 131072 keys 2.4 ms).
 bool kv4_tiles_apply(const AttnArgs &a, int type) {
   const double rows = static_cast<double>(a.max_q) * a.group;
   const double ctas = std::ceil(rows / kRows) * a.Hkv * a.B;

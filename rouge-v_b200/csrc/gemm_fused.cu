@@ -6,8 +6,10 @@
 // activation cost registers only, and overlap the next tile's MMAs
 // (double-buffered accumulator). The residual is read once, by the lanes
 // that round and store the same elements. Measured: int8 16 x 8192 x 8192 with
-// bias and residual 20.1 us (3376 GB/s); bf16 1000 x 14336 x 4096 with gelu, f32
-// out, 108 (1084 TFLOP/s); e4m3 8192^3 with silu and residual 430 (2555).
+// bias and residual 20.1 us (3376 GB/s); int8 4096^3 with the same 60.8 (2262
+// TOP/s; 60.4 without epilogue); bf16 1000 x 14336 x 4096 with gelu, f32 out, 107
+// (1095 TFLOP/s; without gelu 99.7: the last tiles' epilogue is not under any
+// MMA); e4m3 8192^3 with silu and residual 425 to 430 (2555 and more).
 #include "gemm_impl.cuh"
 
 namespace rb200 {

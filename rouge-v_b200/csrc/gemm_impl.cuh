@@ -187,10 +187,12 @@ struct Cfg {
   static constexpr int UMMA_K = 32 / ESIZE;         // elements of K per instruction
   static constexpr int A_BYTES = A_ROWS * kBKBytes;
   static constexpr int B_BYTES = BN * kBKBytes;
-  // k-blocks per stage: a stage's round trip costs 0.13 us whatever it holds,
-  // next to 0.14 us for a few-row k-block (the shared memory's bandwidth:
-  // four MMAs read 24 KB, the copies write 10). M = 16, N = K = 8192, int8:
-  // 24.1 us with one, 20.3 with two, 18.6 with four, 20.2 with eight.
+  // k-blocks per stage: a stage's round trip costs about as much as a few-row
+  // k-block (whose four MMAs read 24 KB of shared memory, the copies write 10).
+  // M = 16, N = K = 8192, int8, empty epilogue: 24.3 us with one, 20.2 with
+  // two, 18.9 with four, 20.2 with eight (with bias and residual 1.3 more each).
+  // Of the 18.9, 4.7 do not depend on K (K = 512: 5.5), the rest is 0.2 us per
+  // k-block, at N = 4096 as at 8192.
   static constexpr int NKB = A_ROWS < kBM ? 4 : 1;
   static constexpr int BLOCK_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGE_BYTES = NKB * BLOCK_BYTES;
@@ -340,9 +342,10 @@ __device__ __forceinline__ void add_residual(const GemmArgs &args, int row, int 
 }
 
 // Activations of the fused epilogue, on f32 sums: gelu is the erf form
-// v/2 (1 + erf(v / sqrt 2)); silu v / (1 + e^-v) with the fast exponential
-// and divide (relative error about 2^-21 |v|, far below the 2^-9 of a bf16
-// output and the 1e-5 of an f32 one).
+// v/2 (1 + erf(v / sqrt 2)), off by up to 2^-22 |v| where 1 + erf cancels;
+// silu v / (1 + e^-v) with the fast exponential and divide (relative error about
+// 2^-21 |v|, far below the 2^-9 of a bf16 output and the 1e-5 of an f32 one;
+// zero for v below -87.3, where the value is below 1e-36).
 __device__ __forceinline__ void apply_act(int act, float (&f)[32]) {
   if (act == ROUGE_B200_ACT_RELU) {
 #pragma unroll

@@ -5,9 +5,10 @@
 // plus one scale byte out (or the reverse). Neighbouring threads hold
 // neighbouring blocks, so a warp reads whole lines of K or V and writes
 // whole sectors of the page. The floor is memory: 2 or 4 bytes in and 0.5625
-// bytes out per value. 32768 bf16 tokens of 8 x 128: 39.2 us to write (67 % of
-// the copy rate; 58 % of the integer pipe, about 200 instructions per thread),
-// 30.8 to read (85 %). Two blocks per thread in flight gained nothing in either.
+// bytes out per value. 32768 bf16 tokens of 8 x 128: 39 to 41 us to write (64 to
+// 67 % of the copy rate; no pipe is full: 64 % of the issue slots, 58 % of the
+// integer pipe, about 200 instructions per thread), 31 to read (84 %). Two
+// blocks per thread in flight gained nothing in either.
 #include <cuda_runtime.h>
 
 #include <cstdint>

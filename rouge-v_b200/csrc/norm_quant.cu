@@ -14,8 +14,10 @@
 // of y -- and the codes, while the block's next row is on its way into other
 // registers. One to 32 warps share a row, so that 512 to 16384 columns fit;
 // longer rows take the looping kernel, which reads h again. With residual: 4096
-// x 4096 f32 to int8 41.2 us, 8191 x 8192 bf16 to MXFP8 85.6 (81 and 84 % of
-// the copy rate); the latter uses 67 % of the issue slots.
+// x 4096 f32 to int8 42 us, 8191 x 8192 bf16 to MXFP8 86 (79 and 84 % of the
+// copy rate); the latter uses 67 % of the issue slots. Wider f32 rows are
+// slower, 4096 x 8192 98 us (68 %): 16 warps a row leave a thread 64 registers,
+// of which the row, the next row and its residual are 48, and 180 bytes spill.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
