@@ -772,3 +772,64 @@ def test_window_counts_from_the_length_past_the_table(rb, cuda, t, nq, Hq):
     hidden = torch.arange(n, device="cuda") >= have
     _close(O, *_sequence_reference(cache, q, n, longer[0], window, hidden, 2.0 ** -32 if nq == 500 else 2.0 ** -40), t,
            have)
+
+
+@pytest.mark.parametrize("t,nq,Hq,Dh", [("f32", 1, 8, 64), ("bf16", 1, 8, 128), ("f16", 7, 8, 96), ("bf16", 500, 16, 128)])
+def test_special_queries_stay_in_their_rows(rb, cuda, t, nq, Hq, Dh):
+    """NaN and infinities in some heads' queries: those rows are NaN, the others as without them."""
+    import torch
+    n = 520
+    cache = _cache(rb, 33, 4, 16, Dh, nq)
+    g = torch.Generator("cuda").manual_seed(nq)
+    table = torch.randperm(33, generator=g, device="cuda").int()[None]
+    q = torch.randn(nq, Hq, Dh, generator=g, device="cuda").to(_dt(t))
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, nq], dtype=torch.int32, device="cuda")
+    run = lambda x: rb.attention_kv4(x, cache, lens, table, cu_q=cu, max_q=nq)  # noqa: E731
+    good = run(q)
+    odd = q.clone()
+    odd[0, 0, 3], odd[nq // 2, 5, Dh - 1], odd[nq - 1, 2, :] = math.nan, math.inf, -math.inf
+    O = run(odd)
+    rb.sync_status()
+    hit = torch.zeros(nq, Hq, dtype=torch.bool, device="cuda")
+    hit[0, 0] = hit[nq // 2, 5] = hit[nq - 1, 2] = True
+    assert O[hit].isnan().all() and torch.equal(O[~hit], good[~hit])
+
+
+def test_decoder_step_in_f32(rb, cuda):
+    """The chain with f32 queries, keys and values, which quantize_i8_rows takes from the attention as they are."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(1)
+    T, D, Hq, Hkv, Dh, page = 9, 512, 8, 2, 64, 16
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    i8 = lambda *s: torch.empty(*s, dtype=torch.int8, device="cuda")  # noqa: E731
+    N = (Hq + 2 * Hkv) * Dh
+
+    def q8(w):
+        q, s = i8(*w.shape), torch.empty(w.shape[0], device="cuda")
+        rb.quantize_i8_rows(w.contiguous(), s, q)
+        return q, s
+    (wqkv, sw), (wo, swo) = q8(rn(N, D) / 23), q8(rn(D, Hq * Dh) / 23)
+    w, bias = 0.5 + torch.rand(D, generator=g, device="cuda"), rn(N)
+    cache = rb.KV4Cache.empty(4, Hkv, page, Dh)
+    x, r, h = rn(T, D).bfloat16(), rn(T, D).bfloat16(), torch.empty(T, D, dtype=torch.bfloat16, device="cuda")
+    qx, sx = i8(T, D), torch.empty(T, device="cuda")
+    rb.add_rmsnorm_quant(x, r, w, 1e-5, rb.Q_I8_ROWS, qx, sx, h)
+    qkv = torch.empty(T, N, device="cuda")
+    rb.gemm_i8(qx, wqkv, rb.B_NK, qkv, rb.OUT_F32, sx, 1, sw, 1, epilogue=rb.Epilogue(bias))
+    k, v = (qkv[:, a * Dh:(a + Hkv) * Dh].unflatten(1, (Hkv, Dh)) for a in (Hq, Hq + Hkv))
+    rb.kv4_write(cache, k, v, torch.arange(16, 16 + T, dtype=torch.int32, device="cuda"))
+    q = qkv[:, :Hq * Dh].reshape(T, Hq, Dh).contiguous()
+    table = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    att = rb.attention_kv4(q, cache, torch.tensor([T], dtype=torch.int32, device="cuda"), table, max_q=T,
+                           cu_q=torch.tensor([0, T], dtype=torch.int32, device="cuda"))
+    o8, so = q8(att.reshape(T, Hq * Dh))
+    out = h.clone()
+    rb.gemm_i8(o8, wo, rb.B_NK, out, rb.OUT_BF16, so, 1, swo, 1, epilogue=rb.Epilogue(residual=out))
+    rb.sync_status()
+    wq = (qx.double() @ wqkv.double().T) * sx.double()[:, None] * sw.double()
+    assert ((qkv.double() - wq - bias.double()).abs() <= 2.0 ** -22 * (wq.abs() + bias.double().abs())).all()
+    hidden = torch.zeros(T, dtype=torch.bool, device="cuda")
+    _close(att, *_sequence_reference(cache, q, T, table[0], 0, hidden, 2.0 ** -40), "f32", T)
+    wo_ = (o8.double() @ wo.double().T) * so.double()[:, None] * swo.double() + h.double()
+    assert ((out.double() - wo_).abs() <= wo_.abs() * 2.0 ** -8 + 2.0 ** -20).all()
