@@ -833,3 +833,30 @@ def test_decoder_step_in_f32(rb, cuda):
     _close(att, *_sequence_reference(cache, q, T, table[0], 0, hidden, 2.0 ** -40), "f32", T)
     wo_ = (o8.double() @ wo.double().T) * so.double()[:, None] * swo.double() + h.double()
     assert ((out.double() - wo_).abs() <= wo_.abs() * 2.0 ** -8 + 2.0 ** -20).all()
+
+
+def test_cache_offsets_past_32_bits(rb, cuda):
+    """Pages whose codes lie past 2^32 bytes: written, read and attended to as the same tokens in a small cache."""
+    import torch
+    Hkv, page, Dh, pages, n = 8, 64, 128, 135000, 700   # 4.4 GB of codes each for keys and values
+    big, small = rb.KV4Cache.empty(pages, Hkv, page, Dh), rb.KV4Cache.empty(12, Hkv, page, Dh)
+    assert big.tensors[0].numel() > 1 << 32
+    g = torch.Generator("cuda").manual_seed(7)
+    K, V = (torch.randn(n, Hkv, Dh, generator=g, device="cuda").bfloat16() for _ in range(2))
+    at = torch.arange(n, dtype=torch.int32, device="cuda")
+    per = -(-n // page)
+    rb.kv4_write(small, K, V, at)
+    rb.kv4_write(big, K, V, at + (pages - per) * page)
+    outs = [torch.empty_like(K) for _ in range(4)]
+    rb.kv4_read(small, at, *outs[:2])
+    rb.kv4_read(big, at + (pages - per) * page, *outs[2:])
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    low = torch.arange(per, dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for nq in (1, 5, 400):
+        q = torch.randn(nq, 16, Dh, generator=g, device="cuda").bfloat16()
+        cu = torch.tensor([0, nq], dtype=torch.int32, device="cuda")
+        a, b = (rb.attention_kv4(q, c, lens, (low + first).contiguous(), cu_q=cu, max_q=nq)
+                for c, first in ((small, 0), (big, pages - per)))
+        assert torch.equal(a, b) and a.float().abs().max() > 0.01
+    rb.sync_status()
